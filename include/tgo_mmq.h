@@ -41,6 +41,15 @@ extern "C" {
 #define TGO_Q6_K 14
 #define TGO_IQ2_S 22
 
+/* Types of logits (tgo_moe_router and its kin, tgo_logit_rules) */
+#define TGO_BF16 0
+#define TGO_FP16 1
+#define TGO_FP32 2
+
+/* What the logits of a router are on a logarithmic scale: the scores themselves, or log sigmoid of them */
+#define TGO_SCORING_SOFTMAX 0
+#define TGO_SCORING_SIGMOID 1
+
 /* Most tiles (rows / 256 + groups) tgo_grouped_fwd_noalloc accepts. */
 #define TGO_NOALLOC_MAX_TILES 4096
 
@@ -344,6 +353,74 @@ int tgo_swiglu_fwd(const void* gate, const void* up, const float* row_scale, voi
 int tgo_swiglu_bwd(const void* dh, const void* gate, const void* up, const float* row_scale,
                    void* dgate, void* dup, int64_t rows, int64_t width,
                    const int32_t* n_rows_device, void* stream);
+
+/* ---- routing of a mixture-of-experts layer (no counterpart in the reference, whose grouped calls take
+ * rows sorted by expert: csrc/mmq_hip.cu:325-406).  logits [tokens][experts] of type `dtype` (TGO_BF16,
+ * TGO_FP16, TGO_FP32), rows row_stride elements apart; experts <= 1024, top_k <= 32.  u = logit
+ * (TGO_SCORING_SOFTMAX) or log sigmoid(logit) (TGO_SCORING_SIGMOID). */
+
+/* expert_ids int32 [tokens][top_k]: the top_k largest logits of a token, largest first, of equal ones the
+ * lower expert first; -1 where only -inf and NaN are left, and for tokens whose token_mask byte is 0 (null:
+ * every token counts; logits of a token that does not are not looked at).  weights fp32 [tokens][top_k]:
+ * normalize: softmax of u over the chosen; else softmax of the logits over all experts, or sigmoid(logit).
+ * 0 beside expert -1; NaN in a row with a NaN among its logits (or, softmax, with +inf). */
+int tgo_moe_router(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t row_stride, int64_t top_k,
+                   int scoring, int normalize, const uint8_t* token_mask, float* weights, int32_t* expert_ids, void* stream);
+
+/* d_logits [tokens][experts], type `dtype`, from the cotangent of the weights; expert_ids and weights are
+ * what tgo_moe_router gave. */
+int tgo_moe_router_grad(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t row_stride,
+                        const int32_t* expert_ids, const float* weights, const float* d_weights, int64_t top_k, int scoring,
+                        int normalize, void* d_logits, void* stream);
+
+/* loss = experts * sum_e f_e P_e: f_e = share of the pairs (token, expert id) that name e, P_e = mean over
+ * the tokens of softmax(u)_e; 1 for an even use.  Ids outside 0..experts-1 name nothing; a token all of whose
+ * ids are such takes no part (its logits are not looked at).  No tokens left: 0.  counts int32 [experts]: pairs
+ * of each expert.  coef fp32 [experts]: what tgo_moe_balance_grad needs of them. */
+int64_t tgo_moe_balance_workspace_bytes(int64_t tokens, int64_t experts);
+int tgo_moe_balance_loss(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t row_stride,
+                         const int32_t* expert_ids, int64_t top_k, int scoring, float* loss, int32_t* counts, float* coef,
+                         void* workspace, int64_t workspace_bytes, void* stream);
+/* d_logits [tokens][experts], type `dtype`, for the cotangent *d_loss (device); the counts are constants. */
+int tgo_moe_balance_grad(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t row_stride,
+                         const int32_t* expert_ids, int64_t top_k, int scoring, const float* coef, const float* d_loss,
+                         void* d_logits, void* stream);
+
+/* Token rows x [tokens][width] (bf16, width a multiple of 8) to rows sorted by expert, pairs of one expert in
+ * their order: rows [tokens * top_k][width], row_of_pair int32 [tokens][top_k] (-1: the pair's id names no
+ * expert), expert_indices / expert_offsets as the grouped calls take them.  Rows behind the last expert's are
+ * zeros. */
+int64_t tgo_moe_dispatch_workspace_bytes(int64_t n_pairs, int64_t num_experts);
+int tgo_moe_dispatch(const void* x, const int32_t* expert_ids, int64_t tokens, int64_t top_k, int64_t num_experts, int64_t width,
+                     void* rows, int32_t* row_of_pair, int64_t* expert_indices, int32_t* expert_offsets, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+
+/* out[t] = sum_s weights[t][s] * rows[row_of_pair[t][s]] (null weights: 1; fp32 sums, one rounding); pairs whose
+ * row is outside 0..n_rows-1 add nothing. */
+int tgo_moe_combine(const void* rows, int64_t n_rows, const int32_t* row_of_pair, const float* weights, void* out, int64_t tokens,
+                    int64_t top_k, int64_t width, void* stream);
+/* Its gradients: d_rows [n_rows][width] (null: not wanted; zeros where no pair names the row, the sum where several
+ * do) and d_weights fp32 [tokens][top_k] (null: not wanted; 0 for pairs without a row; needs rows).  workspace:
+ * n_rows * 4 bytes if d_rows is wanted. */
+int tgo_moe_combine_grad(const void* dy, const void* rows, int64_t n_rows, const int32_t* row_of_pair, const float* weights,
+                         void* d_rows, float* d_weights, int64_t tokens, int64_t top_k, int64_t width, void* workspace,
+                         int64_t workspace_bytes, void* stream);
+
+/* ---- rules on the logits of a generation step (no counterpart in the reference).  Row by row, in fp32:
+ *   x = logit + sum of the biases that name the token;
+ *   c = occurrences of the token in the first lengths[row] of the row's history_len ids; where c > 0:
+ *       x = (x > 0 ? x / repetition : x * repetition) - (c * frequency + presence);
+ *   x = -inf where bit (token % 32) of allowed[row][token / 32] is 0;
+ * one rounding to `dtype`.  out may be logits itself (with the same strides).  Null: history (nothing is
+ * penalised), lengths (all history_len ids), allowed (every token), bias_ids (none); repetition, presence,
+ * frequency (fp32 [rows]; null: the value beside them).  Ids of 4 or 8 bytes; those outside the vocabulary name
+ * nothing.  Strides in elements; a stride of 0 gives every row the same ids or mask. */
+int tgo_logit_rules(const void* logits, void* out, int dtype, int64_t rows, int64_t vocab, int64_t in_stride, int64_t out_stride,
+                    const void* history, const void* lengths, int64_t history_len, int64_t history_stride, int history_id_bytes,
+                    int length_bytes, const float* repetition, float repetition_all, const float* presence, float presence_all,
+                    const float* frequency, float frequency_all, const void* bias_ids, const float* bias_values, int64_t n_bias,
+                    int64_t bias_ids_stride, int64_t bias_values_stride, int bias_id_bytes, const uint32_t* allowed,
+                    int64_t allowed_stride, void* stream);
 
 /* Grouped forward for callers that cannot hand over a workspace and must not trigger a device
  * allocation: the same operation and results as tgo_grouped_fwd, with the tile list kept in a

@@ -146,10 +146,10 @@ def build_shim(force: bool = False) -> Path:
 def build_ext(force: bool = False) -> Path:
     import torch
 
-    src = CSRC / "torch_ext.cpp"
+    srcs = sorted(CSRC.glob("torch_ext*.cpp"))
     # libtorch's C++ ABI holds for one torch release, so the release is part of what the module is built from
     built_for = BUILD / "torch_ext.torch_version"
-    if not force and _newer(EXT_PATH, [src, ROOT / "include" / "tgo_mmq.h", LIB_PATH]) and built_for.exists() \
+    if not force and _newer(EXT_PATH, [*srcs, CSRC / "torch_ext.h", ROOT / "include" / "tgo_mmq.h", LIB_PATH]) and built_for.exists() \
             and built_for.read_text() == torch.__version__:
         return EXT_PATH
     tdir = Path(torch.__file__).resolve().parent
@@ -158,7 +158,7 @@ def build_ext(force: bool = False) -> Path:
            cuda / "include"]
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     _run([_host_cxx(), "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DPy_LIMITED_API=0x030A0000",
-          *[f"-I{p}" for p in inc], str(src), "-o", str(EXT_PATH),
+          *[f"-I{p}" for p in inc], *map(str, srcs), "-o", str(EXT_PATH),
           f"-L{LIB_DIR}", "-ltgo_mmq", f"-L{tdir / 'lib'}", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda",
           "-Wl,-rpath,$ORIGIN/lib", f"-Wl,-rpath,{tdir / 'lib'}"])
     BUILD.mkdir(parents=True, exist_ok=True)

@@ -1,6 +1,7 @@
 // The parts of the operator surface that need libtorch's C++ API: the autograd formulas of the six
 // reference operators (their CUDA kernels are registered through the stable ABI, torch_shim.cpp) and
-// this package's own operators mmq_multi, swiglu and lm_head_loss with theirs.
+// this package's own operators mmq_multi, swiglu and lm_head_loss with theirs (the routing operators and
+// logit_rules: torch_ext_routing.cpp).
 //
 // Why not in Python: a formula registered there costs a call into the interpreter for every operator
 // call, some 5 us without and 50 us with a gradient, against 8 to 60 us of kernel in a decode step or a
@@ -9,30 +10,15 @@
 // operators refuse a second derivative.
 #include <Python.h>
 
-#include <ATen/ATen.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <c10/cuda/CUDAStream.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/library.h>
-
 #include <algorithm>
 #include <cmath>
 
-#include "../../include/tgo_mmq.h"
+#include "torch_ext.h"
 
 namespace {
 
-using at::Tensor;
-using torch::autograd::AutogradContext;
-using torch::autograd::Function;
-using torch::autograd::tensor_list;
-using torch::autograd::Variable;
-using torch::autograd::variable_list;
+using namespace tgo_ext;
 
-template <typename Fn>
-const c10::TypedOperatorHandle<Fn> op(const char* name) {
-    return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Fn>();
-}
 // the last dimension as a plain integer (a traced shape is specialised on it, as an int argument is)
 int64_t last_size(const Tensor& t, int64_t dim) { return t.sym_size(dim).guard_int(__FILE__, __LINE__); }
 
@@ -65,7 +51,6 @@ Tensor call_pair_dx(const Tensor& d0, const Tensor& d1, const Tensor& w0, const 
     return h.call(d0, d1, w0, w1, ei, eo, qt, k);
 }
 
-bool wants_grad(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 // A cotangent handed over by autograd may be a transposed view; the operators refuse what is not
 // contiguous.  (One that starts inside a storage stays as it is, and is refused.)
 Tensor plain(const Tensor& g) { return g.contiguous(); }
@@ -195,9 +180,6 @@ Tensor pair_dx_autograd(const Tensor& d0, const Tensor& d1, const Tensor& w0, co
 }
 
 // ------------------------------------------------------------------ mmq_multi
-void check_rc(int rc, const char* what) { TORCH_CHECK(rc == TGO_OK, what, " failed: ", tgo_last_error()); }
-void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
-
 void check_activation(const Tensor& t, const char* name) {
     TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
     TORCH_CHECK(t.scalar_type() == at::kBFloat16 && t.is_contiguous() && t.storage_offset() == 0, name,

@@ -1,0 +1,524 @@
+// Operators either side of the experts' products and of the head's, over libtorch's C++ API as in
+// torch_ext.cpp: the router of a mixture-of-experts layer, its balance loss, rows sorted by expert and back
+// (moe_router, moe_balance_loss, moe_dispatch, moe_combine, with their gradients) and the rules on a
+// generation step's logits (logit_rules).
+#include <ATen/MemoryOverlap.h>
+
+#include "torch_ext.h"
+
+namespace {
+
+using namespace tgo_ext;
+
+int type_code(const Tensor& logits) {
+    switch (logits.scalar_type()) {
+        case at::kBFloat16: return TGO_BF16;
+        case at::kHalf: return TGO_FP16;
+        case at::kFloat: return TGO_FP32;
+        default: TORCH_CHECK(false, "logits must have dtype torch.bfloat16, torch.float16 or torch.float32; got ", logits.scalar_type());
+    }
+}
+// [..., width] as rows: a matrix whose rows may lie apart, or anything contiguous
+struct Rows {
+    int64_t rows, width, stride;
+};
+Rows as_rows(const Tensor& t, const char* name) {
+    TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+    TORCH_CHECK(t.dim() >= 1, name, " must have at least one dimension");
+    const int64_t width = t.size(-1);
+    TORCH_CHECK(width > 0, name, " must not be empty in its last dimension");
+    const int64_t rows = t.numel() / width;
+    if (t.is_contiguous()) return {rows, width, width};
+    TORCH_CHECK(t.dim() == 2 && (width == 1 || t.stride(1) == 1) && t.stride(0) >= width, name,
+                " must be contiguous, or a matrix whose rows lie apart; torch_ggml_ops will not insert a hidden copy");
+    return {rows, width, t.stride(0)};
+}
+void check_plain(const Tensor& t, const Tensor& like, at::ScalarType type, const char* name) {
+    TORCH_CHECK(t.device() == like.device() && t.scalar_type() == type && t.is_contiguous(), name, " must be a contiguous ", type,
+                " tensor on the other inputs' device; torch_ggml_ops will not insert a hidden copy");
+}
+std::vector<int64_t> with_last(at::IntArrayRef sizes, int64_t last) {
+    std::vector<int64_t> v = sizes.vec();
+    v.back() = last;
+    return v;
+}
+
+// ------------------------------------------------------------------ moe_router
+void check_router(const Rows& r, int64_t top_k, int64_t scoring) {
+    TORCH_CHECK(r.width <= 1024, "the router takes up to 1024 experts; got ", r.width);
+    TORCH_CHECK(top_k >= 1 && top_k <= 32 && top_k <= r.width, "top_k must be in 1..32 and at most the number of experts; got ", top_k);
+    TORCH_CHECK(scoring == TGO_SCORING_SOFTMAX || scoring == TGO_SCORING_SIGMOID, "unknown scoring");
+}
+std::tuple<Tensor, Tensor> router_cuda(const Tensor& logits, int64_t top_k, int64_t scoring, bool normalize, const std::optional<Tensor>& mask) {
+    const int code = type_code(logits);
+    const Rows r = as_rows(logits, "logits");
+    check_router(r, top_k, scoring);
+    if (mask.has_value()) {
+        check_plain(*mask, logits, at::kBool, "token_mask");
+        TORCH_CHECK(mask->sizes() == logits.sizes().slice(0, logits.dim() - 1), "token_mask must have one entry per token");
+    }
+    const c10::cuda::CUDAGuard guard(logits.device());
+    const auto sizes = with_last(logits.sizes(), top_k);
+    Tensor w = at::empty(sizes, logits.options().dtype(at::kFloat)), ids = at::empty(sizes, logits.options().dtype(at::kInt));
+    if (r.rows > 0)
+        check_rc(tgo_moe_router(logits.const_data_ptr(), code, r.rows, r.width, r.stride, top_k, static_cast<int>(scoring), normalize,
+                                mask.has_value() ? reinterpret_cast<const uint8_t*>(mask->const_data_ptr<bool>()) : nullptr,
+                                w.mutable_data_ptr<float>(), ids.mutable_data_ptr<int32_t>(), stream_of(logits)),
+                 "moe_router");
+    return {w, ids};
+}
+Tensor router_grad_cuda(const Tensor& grad, const Tensor& logits, const Tensor& ids, const Tensor& w, int64_t scoring, bool normalize) {
+    const int code = type_code(logits);
+    const Rows r = as_rows(logits, "logits");
+    check_plain(ids, logits, at::kInt, "expert_ids");
+    check_plain(w, logits, at::kFloat, "weights");
+    TORCH_CHECK(grad.sizes() == w.sizes() && grad.scalar_type() == at::kFloat && grad.device() == w.device() && ids.sizes() == w.sizes() &&
+                    w.dim() == logits.dim() && w.sizes().slice(0, w.dim() - 1) == logits.sizes().slice(0, w.dim() - 1),
+                "grad, expert_ids and weights must be tensors of one shape, one row per token");
+    check_router(r, w.size(-1), scoring);
+    const c10::cuda::CUDAGuard guard(logits.device());
+    const Tensor d = grad.contiguous();
+    Tensor dx = at::empty(logits.sizes(), logits.options());
+    if (r.rows > 0)
+        check_rc(tgo_moe_router_grad(logits.const_data_ptr(), code, r.rows, r.width, r.stride, ids.const_data_ptr<int32_t>(),
+                                     w.const_data_ptr<float>(), d.const_data_ptr<float>(), w.size(-1), static_cast<int>(scoring), normalize,
+                                     dx.mutable_data_ptr(), stream_of(logits)),
+                 "moe_router_grad");
+    return dx;
+}
+std::tuple<Tensor, Tensor> call_router(const Tensor& x, int64_t k, int64_t scoring, bool norm, const std::optional<Tensor>& mask) {
+    static const auto h = op<std::tuple<Tensor, Tensor>(const Tensor&, int64_t, int64_t, bool, const std::optional<Tensor>&)>(
+        "torch_ggml_ops_b200::moe_router");
+    return h.call(x, k, scoring, norm, mask);
+}
+Tensor call_router_grad(const Tensor& g, const Tensor& x, const Tensor& ids, const Tensor& w, int64_t scoring, bool norm) {
+    static const auto h = op<Tensor(const Tensor&, const Tensor&, const Tensor&, const Tensor&, int64_t, bool)>(
+        "torch_ggml_ops_b200::moe_router_grad");
+    return h.call(g, x, ids, w, scoring, norm);
+}
+[[noreturn]] void once_only(const char* name) {
+    TORCH_CHECK(false, "torch_ggml_ops_b200::", name, " does not support higher-order gradients");
+}
+struct RouterFn : public Function<RouterFn> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, int64_t k, int64_t scoring, bool norm, const std::optional<Tensor>& mask) {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        auto [w, ids] = call_router(x, k, scoring, norm, mask);
+        ctx->save_for_backward({x, ids, w});
+        ctx->saved_data["scoring"] = scoring;
+        ctx->saved_data["norm"] = norm;
+        ctx->mark_non_differentiable({ids});
+        ctx->set_materialize_grads(false);
+        return {w, ids};
+    }
+    static tensor_list backward(AutogradContext* ctx, tensor_list g) {
+        Tensor dx;
+        if (ctx->needs_input_grad(0) && g[0].defined()) {
+            const variable_list s = ctx->get_saved_variables();
+            dx = call_router_grad(g[0], s[0], s[1], s[2], ctx->saved_data["scoring"].toInt(), ctx->saved_data["norm"].toBool());
+        }
+        return {dx, Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+std::tuple<Tensor, Tensor> router_autograd(const Tensor& x, int64_t k, int64_t scoring, bool norm, const std::optional<Tensor>& mask) {
+    if (wants_grad(x)) {
+        const variable_list r = RouterFn::apply(x, k, scoring, norm, mask);
+        return {r[0], r[1]};
+    }
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return call_router(x, k, scoring, norm, mask);
+}
+struct RouterGradFn : public Function<RouterGradFn> {
+    static Tensor forward(AutogradContext*, const Tensor& g, const Tensor& x, const Tensor& ids, const Tensor& w, int64_t scoring, bool norm) {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        return call_router_grad(g, x, ids, w, scoring, norm);
+    }
+    static tensor_list backward(AutogradContext*, tensor_list) { once_only("moe_router_grad"); }
+};
+Tensor router_grad_autograd(const Tensor& g, const Tensor& x, const Tensor& ids, const Tensor& w, int64_t scoring, bool norm) {
+    if (wants_grad(g) || wants_grad(x) || wants_grad(w)) return RouterGradFn::apply(g, x, ids, w, scoring, norm);
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return call_router_grad(g, x, ids, w, scoring, norm);
+}
+
+// ------------------------------------------------------------------ moe_balance_loss
+void check_ids(const Tensor& ids, const Tensor& tokens, const char* of) {
+    check_plain(ids, tokens, at::kInt, "expert_ids");
+    TORCH_CHECK(ids.dim() == tokens.dim() && ids.sizes().slice(0, ids.dim() - 1) == tokens.sizes().slice(0, ids.dim() - 1),
+                "expert_ids must have one row per row of ", of);
+}
+std::tuple<Tensor, Tensor, Tensor> balance_cuda(const Tensor& logits, const Tensor& ids, int64_t scoring) {
+    const int code = type_code(logits);
+    const Rows r = as_rows(logits, "logits");
+    check_ids(ids, logits, "logits");
+    check_router(r, ids.size(-1), scoring);
+    const c10::cuda::CUDAGuard guard(logits.device());
+    const auto f32 = logits.options().dtype(at::kFloat);
+    if (r.rows == 0) return {at::zeros({}, f32), at::zeros({r.width}, f32.dtype(at::kInt)), at::zeros({r.width}, f32)};
+    Tensor loss = at::empty({}, f32), counts = at::empty({r.width}, f32.dtype(at::kInt)), coef = at::empty({r.width}, f32);
+    const int64_t bytes = tgo_moe_balance_workspace_bytes(r.rows, r.width);
+    TORCH_CHECK(bytes >= 0, "unsupported sizes");
+    Tensor ws = at::empty({bytes}, f32.dtype(at::kByte));
+    check_rc(tgo_moe_balance_loss(logits.const_data_ptr(), code, r.rows, r.width, r.stride, ids.const_data_ptr<int32_t>(), ids.size(-1),
+                                  static_cast<int>(scoring), loss.mutable_data_ptr<float>(), counts.mutable_data_ptr<int32_t>(),
+                                  coef.mutable_data_ptr<float>(), ws.mutable_data_ptr(), bytes, stream_of(logits)),
+             "moe_balance_loss");
+    return {loss, counts, coef};
+}
+Tensor balance_grad_cuda(const Tensor& grad, const Tensor& logits, const Tensor& ids, const Tensor& coef, int64_t scoring) {
+    const int code = type_code(logits);
+    const Rows r = as_rows(logits, "logits");
+    check_ids(ids, logits, "logits");
+    check_router(r, ids.size(-1), scoring);
+    check_plain(coef, logits, at::kFloat, "coef");
+    TORCH_CHECK(coef.numel() == r.width, "coef must have one entry per expert");
+    check_plain(grad, logits, at::kFloat, "grad");
+    TORCH_CHECK(grad.numel() == 1, "grad must be one number");
+    const c10::cuda::CUDAGuard guard(logits.device());
+    Tensor dx = at::empty(logits.sizes(), logits.options());
+    if (r.rows > 0)
+        check_rc(tgo_moe_balance_grad(logits.const_data_ptr(), code, r.rows, r.width, r.stride, ids.const_data_ptr<int32_t>(), ids.size(-1),
+                                      static_cast<int>(scoring), coef.const_data_ptr<float>(), grad.const_data_ptr<float>(),
+                                      dx.mutable_data_ptr(), stream_of(logits)),
+                 "moe_balance_grad");
+    return dx;
+}
+std::tuple<Tensor, Tensor, Tensor> call_balance(const Tensor& x, const Tensor& ids, int64_t scoring) {
+    static const auto h = op<std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, int64_t)>("torch_ggml_ops_b200::moe_balance_loss");
+    return h.call(x, ids, scoring);
+}
+Tensor call_balance_grad(const Tensor& g, const Tensor& x, const Tensor& ids, const Tensor& coef, int64_t scoring) {
+    static const auto h = op<Tensor(const Tensor&, const Tensor&, const Tensor&, const Tensor&, int64_t)>("torch_ggml_ops_b200::moe_balance_grad");
+    return h.call(g, x, ids, coef, scoring);
+}
+struct BalanceFn : public Function<BalanceFn> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& ids, int64_t scoring) {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        auto [loss, counts, coef] = call_balance(x, ids, scoring);
+        ctx->save_for_backward({x, ids, coef});
+        ctx->saved_data["scoring"] = scoring;
+        ctx->mark_non_differentiable({counts, coef});
+        ctx->set_materialize_grads(false);
+        return {loss, counts, coef};
+    }
+    static tensor_list backward(AutogradContext* ctx, tensor_list g) {
+        Tensor dx;
+        if (ctx->needs_input_grad(0) && g[0].defined()) {
+            const variable_list s = ctx->get_saved_variables();
+            dx = call_balance_grad(g[0], s[0], s[1], s[2], ctx->saved_data["scoring"].toInt());
+        }
+        return {dx, Tensor(), Tensor()};
+    }
+};
+std::tuple<Tensor, Tensor, Tensor> balance_autograd(const Tensor& x, const Tensor& ids, int64_t scoring) {
+    if (wants_grad(x)) {
+        const variable_list r = BalanceFn::apply(x, ids, scoring);
+        return {r[0], r[1], r[2]};
+    }
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return call_balance(x, ids, scoring);
+}
+struct BalanceGradFn : public Function<BalanceGradFn> {
+    static Tensor forward(AutogradContext*, const Tensor& g, const Tensor& x, const Tensor& ids, const Tensor& coef, int64_t scoring) {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        return call_balance_grad(g, x, ids, coef, scoring);
+    }
+    static tensor_list backward(AutogradContext*, tensor_list) { once_only("moe_balance_grad"); }
+};
+Tensor balance_grad_autograd(const Tensor& g, const Tensor& x, const Tensor& ids, const Tensor& coef, int64_t scoring) {
+    if (wants_grad(g) || wants_grad(x)) return BalanceGradFn::apply(g, x, ids, coef, scoring);
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return call_balance_grad(g, x, ids, coef, scoring);
+}
+
+// ------------------------------------------------------------------ moe_dispatch and moe_combine
+void check_moved(const Tensor& t, const char* name) {
+    TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+    TORCH_CHECK(t.scalar_type() == at::kBFloat16 && t.is_contiguous() && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0, name,
+                " must be a contiguous torch.bfloat16 tensor that starts at a multiple of 16 bytes; torch_ggml_ops will not insert a hidden copy");
+    TORCH_CHECK(t.dim() >= 1 && t.size(-1) > 0 && t.size(-1) % 8 == 0, name, " must have rows whose length is a positive multiple of 8");
+}
+void check_pairs(int64_t pairs, int64_t top_k) {
+    TORCH_CHECK(top_k >= 1 && top_k <= 1024, "top_k must be in 1..1024; got ", top_k);
+    TORCH_CHECK(pairs <= INT32_MAX, "tokens * top_k must be below 2^31; got ", pairs);
+}
+std::tuple<Tensor, Tensor, Tensor, Tensor> dispatch_cuda(const Tensor& x, const Tensor& ids, int64_t experts) {
+    check_moved(x, "input");
+    TORCH_CHECK(ids.dim() >= 1, "expert_ids must have one row per row of input");
+    check_ids(ids, x, "input");
+    const int64_t h = x.size(-1), tokens = x.numel() / h, k = ids.size(-1), pairs = ids.numel();
+    check_pairs(pairs, k);
+    TORCH_CHECK(experts >= 1 && experts <= 4096, "num_experts must be in 1..4096; got ", experts);
+    const c10::cuda::CUDAGuard guard(x.device());
+    const auto i32 = ids.options(), i64 = i32.dtype(at::kLong);
+    Tensor rows = at::empty({pairs, h}, x.options()), at_row = at::empty(ids.sizes(), i32);
+    if (pairs == 0) return {rows, at_row, at::arange(experts, i64), at::zeros({experts}, i32)};
+    Tensor indices = at::empty({experts}, i64), offsets = at::empty({experts}, i32);
+    const int64_t bytes = tgo_moe_dispatch_workspace_bytes(pairs, experts);
+    TORCH_CHECK(bytes >= 0, "unsupported sizes");
+    Tensor ws = at::empty({bytes}, i32.dtype(at::kByte));
+    check_rc(tgo_moe_dispatch(x.const_data_ptr(), ids.const_data_ptr<int32_t>(), tokens, k, experts, h, rows.mutable_data_ptr(),
+                              at_row.mutable_data_ptr<int32_t>(), indices.mutable_data_ptr<int64_t>(), offsets.mutable_data_ptr<int32_t>(),
+                              ws.mutable_data_ptr(), bytes, stream_of(x)),
+             "moe_dispatch");
+    return {rows, at_row, indices, offsets};
+}
+void check_combine(const Tensor& rows, const Tensor& at_row, const std::optional<Tensor>& w) {
+    check_moved(rows, "rows");
+    TORCH_CHECK(rows.dim() == 2, "rows must have shape [rows, width]");
+    TORCH_CHECK(rows.size(0) <= INT32_MAX, "too many rows");
+    check_plain(at_row, rows, at::kInt, "row_of_pair");
+    TORCH_CHECK(at_row.dim() >= 1, "row_of_pair must have shape [..., top_k]");
+    check_pairs(at_row.numel(), at_row.size(-1));
+    if (w.has_value()) {
+        check_plain(*w, rows, at::kFloat, "weights");
+        TORCH_CHECK(w->sizes() == at_row.sizes(), "weights must have one entry per pair");
+    }
+}
+Tensor combine_cuda(const Tensor& rows, const Tensor& at_row, const std::optional<Tensor>& w) {
+    check_combine(rows, at_row, w);
+    const int64_t h = rows.size(1), k = at_row.size(-1), tokens = at_row.numel() / k;
+    const c10::cuda::CUDAGuard guard(rows.device());
+    const auto sizes = with_last(at_row.sizes(), h);
+    if (rows.size(0) == 0) return at::zeros(sizes, rows.options());
+    Tensor out = at::empty(sizes, rows.options());
+    if (tokens > 0)
+        check_rc(tgo_moe_combine(rows.const_data_ptr(), rows.size(0), at_row.const_data_ptr<int32_t>(),
+                                 w.has_value() ? w->const_data_ptr<float>() : nullptr, out.mutable_data_ptr(), tokens, k, h, stream_of(rows)),
+                 "moe_combine");
+    return out;
+}
+// an empty tensor in the place of a gradient that is not wanted
+std::tuple<Tensor, Tensor> combine_grad_cuda(const Tensor& grad, const Tensor& rows, const Tensor& at_row, const std::optional<Tensor>& w, bool need_rows,
+                                             bool need_weights) {
+    check_combine(rows, at_row, w);
+    const int64_t h = rows.size(1), k = at_row.size(-1), tokens = at_row.numel() / k;
+    const c10::cuda::CUDAGuard guard(rows.device());
+    TORCH_CHECK(grad.device() == rows.device() && grad.scalar_type() == at::kBFloat16 && grad.dim() == at_row.dim() && grad.size(-1) == h &&
+                    grad.numel() == tokens * h,
+                "grad must be a torch.bfloat16 tensor like the result");
+    Tensor d = grad.contiguous();
+    if (reinterpret_cast<uintptr_t>(d.const_data_ptr()) % 16 != 0) d = d.clone();
+    const auto f32 = rows.options().dtype(at::kFloat);
+    Tensor d_rows = at::empty({need_rows ? rows.size(0) : 0, h}, rows.options());
+    Tensor d_w = need_weights ? at::empty(at_row.sizes(), f32) : at::empty({0}, f32);
+    if (rows.size(0) == 0 || tokens == 0) return {d_rows.zero_(), d_w.zero_()};
+    if (!need_rows && !need_weights) return {d_rows, d_w};
+    const int64_t bytes = need_rows ? rows.size(0) * 4 : 0;
+    Tensor ws = at::empty({bytes}, f32.dtype(at::kByte));
+    check_rc(tgo_moe_combine_grad(d.const_data_ptr(), rows.const_data_ptr(), rows.size(0), at_row.const_data_ptr<int32_t>(),
+                                  w.has_value() ? w->const_data_ptr<float>() : nullptr, need_rows ? d_rows.mutable_data_ptr() : nullptr,
+                                  need_weights ? d_w.mutable_data_ptr<float>() : nullptr, tokens, k, h, bytes > 0 ? ws.mutable_data_ptr() : nullptr,
+                                  bytes, stream_of(rows)),
+             "moe_combine_grad");
+    return {d_rows, d_w};
+}
+std::tuple<Tensor, Tensor, Tensor, Tensor> call_dispatch(const Tensor& x, const Tensor& ids, int64_t experts) {
+    static const auto h = op<std::tuple<Tensor, Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, int64_t)>("torch_ggml_ops_b200::moe_dispatch");
+    return h.call(x, ids, experts);
+}
+Tensor call_combine(const Tensor& rows, const Tensor& at_row, const std::optional<Tensor>& w) {
+    static const auto h = op<Tensor(const Tensor&, const Tensor&, const std::optional<Tensor>&)>("torch_ggml_ops_b200::moe_combine");
+    return h.call(rows, at_row, w);
+}
+std::tuple<Tensor, Tensor> call_combine_grad(const Tensor& g, const Tensor& rows, const Tensor& at_row, const std::optional<Tensor>& w, bool need_rows,
+                                             bool need_weights) {
+    static const auto h = op<std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const std::optional<Tensor>&, bool, bool)>(
+        "torch_ggml_ops_b200::moe_combine_grad");
+    return h.call(g, rows, at_row, w, need_rows, need_weights);
+}
+struct DispatchFn : public Function<DispatchFn> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& ids, int64_t experts) {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        auto [rows, at_row, indices, offsets] = call_dispatch(x, ids, experts);
+        ctx->save_for_backward({at_row});
+        ctx->mark_non_differentiable({at_row, indices, offsets});
+        ctx->set_materialize_grads(false);
+        return {rows, at_row, indices, offsets};
+    }
+    static tensor_list backward(AutogradContext* ctx, tensor_list g) {
+        Tensor dx;
+        if (ctx->needs_input_grad(0) && g[0].defined()) {
+            Tensor d = g[0].contiguous();
+            if (d.is_cuda() && reinterpret_cast<uintptr_t>(d.const_data_ptr()) % 16 != 0) d = d.clone();
+            dx = call_combine(d, ctx->get_saved_variables()[0], std::nullopt);
+        }
+        return {dx, Tensor(), Tensor()};
+    }
+};
+std::tuple<Tensor, Tensor, Tensor, Tensor> dispatch_autograd(const Tensor& x, const Tensor& ids, int64_t experts) {
+    if (wants_grad(x)) {
+        const variable_list r = DispatchFn::apply(x, ids, experts);
+        return {r[0], r[1], r[2], r[3]};
+    }
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return call_dispatch(x, ids, experts);
+}
+struct CombineFn : public Function<CombineFn> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& rows, const Tensor& at_row, const std::optional<Tensor>& w) {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        ctx->save_for_backward({rows, at_row, w.has_value() ? *w : Tensor()});
+        ctx->set_materialize_grads(false);
+        return call_combine(rows, at_row, w);
+    }
+    static tensor_list backward(AutogradContext* ctx, tensor_list g) {
+        Tensor d_rows, d_w;
+        if (g[0].defined()) {
+            const variable_list s = ctx->get_saved_variables();
+            const std::optional<Tensor> w = s[2].defined() ? std::optional<Tensor>(s[2]) : std::nullopt;
+            const bool need_rows = ctx->needs_input_grad(0), need_w = w.has_value() && ctx->needs_input_grad(2);
+            if (need_rows || need_w) {
+                auto [a, b] = call_combine_grad(g[0], s[0], s[1], w, need_rows, need_w);
+                if (need_rows) d_rows = a;
+                if (need_w) d_w = b;
+            }
+        }
+        return {d_rows, Tensor(), d_w};
+    }
+};
+Tensor combine_autograd(const Tensor& rows, const Tensor& at_row, const std::optional<Tensor>& w) {
+    if (wants_grad(rows) || (w.has_value() && wants_grad(*w))) return CombineFn::apply(rows, at_row, w);
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return call_combine(rows, at_row, w);
+}
+struct CombineGradFn : public Function<CombineGradFn> {
+    static variable_list forward(AutogradContext*, const Tensor& g, const Tensor& rows, const Tensor& at_row, const std::optional<Tensor>& w, bool need_rows,
+                                 bool need_weights) {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        auto [a, b] = call_combine_grad(g, rows, at_row, w, need_rows, need_weights);
+        return {a, b};
+    }
+    static tensor_list backward(AutogradContext*, tensor_list) { once_only("moe_combine_grad"); }
+};
+std::tuple<Tensor, Tensor> combine_grad_autograd(const Tensor& g, const Tensor& rows, const Tensor& at_row, const std::optional<Tensor>& w, bool need_rows,
+                                                 bool need_weights) {
+    if (wants_grad(g) || wants_grad(rows) || (w.has_value() && wants_grad(*w))) {
+        const variable_list r = CombineGradFn::apply(g, rows, at_row, w, need_rows, need_weights);
+        return {r[0], r[1]};
+    }
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return call_combine_grad(g, rows, at_row, w, need_rows, need_weights);
+}
+
+// ------------------------------------------------------------------ logit_rules
+using MaybeTensor = std::optional<Tensor>;
+bool is_id(const Tensor& t) { return t.scalar_type() == at::kInt || t.scalar_type() == at::kLong; }
+// [rows, n] (rows may lie apart) or [n] for every row: the distance of its rows
+int64_t row_stride(const Tensor& t, const Tensor& logits, int64_t rows, const char* name) {
+    TORCH_CHECK(t.device() == logits.device(), name, " must be on the logits' device");
+    TORCH_CHECK(t.dim() == 1 || (t.dim() == 2 && t.size(0) == rows), name, " must have one row per row of logits, or be one row for all of them");
+    const int64_t n = t.size(-1);
+    TORCH_CHECK(n <= 1 || t.stride(-1) == 1, name, " must be contiguous in its last dimension; torch_ggml_ops will not insert a hidden copy");
+    return t.dim() == 2 ? t.stride(0) : 0;
+}
+const float* per_row(const MaybeTensor& t, const Tensor& logits, int64_t rows, const char* name) {
+    if (!t.has_value()) return nullptr;
+    check_plain(*t, logits, at::kFloat, name);
+    TORCH_CHECK(t->dim() == 1 && t->size(0) == rows, name, " must be a number or have one entry per row of logits");
+    return t->const_data_ptr<float>();
+}
+void rules_into(const Tensor& logits, const MaybeTensor& history, const MaybeTensor& lengths, const MaybeTensor& repetition, double repetition_all,
+                const MaybeTensor& presence, double presence_all, const MaybeTensor& frequency, double frequency_all, const MaybeTensor& bias_ids,
+                const MaybeTensor& bias_values, const MaybeTensor& allowed, const Tensor& out) {
+    const int code = type_code(logits);
+    const Rows r = as_rows(logits, "logits"), o = as_rows(out, "out");
+    TORCH_CHECK(logits.dim() <= 2, "logits must have shape [rows, vocab] or [vocab]");
+    TORCH_CHECK(out.sizes() == logits.sizes() && out.scalar_type() == logits.scalar_type() && out.device() == logits.device(),
+                "out must be a tensor like logits");
+    TORCH_CHECK(r.width <= INT32_MAX, "the vocabulary must be below 2^31; got ", r.width);
+    TORCH_CHECK(repetition.has_value() || repetition_all > 0, "repetition_penalty must be positive; got ", repetition_all);
+    int64_t history_stride = 0, ids_stride = 0, values_stride = 0, allowed_stride = 0;
+    if (history.has_value()) {
+        TORCH_CHECK(is_id(*history), "history must have dtype torch.int32 or torch.int64");
+        history_stride = row_stride(*history, logits, r.rows, "history");
+    }
+    if (lengths.has_value()) {
+        TORCH_CHECK(history.has_value(), "history_lengths need a history");
+        TORCH_CHECK(is_id(*lengths) && lengths->dim() == 1 && lengths->size(0) == r.rows && lengths->is_contiguous() && lengths->device() == logits.device(),
+                    "history_lengths must be a contiguous torch.int32 or torch.int64 tensor with one entry per row of logits");
+    }
+    const float* rep = per_row(repetition, logits, r.rows, "repetition_penalty");
+    const float* pres = per_row(presence, logits, r.rows, "presence_penalty");
+    const float* freq = per_row(frequency, logits, r.rows, "frequency_penalty");
+    TORCH_CHECK(bias_ids.has_value() == bias_values.has_value(), "bias_ids and bias_values come together");
+    if (bias_ids.has_value()) {
+        TORCH_CHECK(is_id(*bias_ids), "bias_ids must have dtype torch.int32 or torch.int64");
+        TORCH_CHECK(bias_values->scalar_type() == at::kFloat, "bias_values must have dtype torch.float32");
+        ids_stride = row_stride(*bias_ids, logits, r.rows, "bias_ids");
+        values_stride = row_stride(*bias_values, logits, r.rows, "bias_values");
+        TORCH_CHECK(bias_ids->size(-1) == bias_values->size(-1), "bias_ids and bias_values must have the same length");
+    }
+    if (allowed.has_value()) {
+        TORCH_CHECK(allowed->scalar_type() == at::kInt, "allowed must have dtype torch.int32");
+        allowed_stride = row_stride(*allowed, logits, r.rows, "allowed");
+        TORCH_CHECK(allowed->size(-1) >= (r.width + 31) / 32, "allowed must have one bit per token: ", (r.width + 31) / 32, " words a row; got ",
+                    allowed->size(-1));
+    }
+    if (r.rows == 0) return;
+    const c10::cuda::CUDAGuard guard(logits.device());
+    const bool some = history.has_value() && history->size(-1) > 0, biased = bias_ids.has_value() && bias_ids->size(-1) > 0;
+    check_rc(tgo_logit_rules(logits.const_data_ptr(), out.mutable_data_ptr(), code, r.rows, r.width, r.stride, o.stride,
+                             some ? history->const_data_ptr() : nullptr, some && lengths.has_value() ? lengths->const_data_ptr() : nullptr,
+                             some ? history->size(-1) : 0, history_stride, some ? static_cast<int>(history->element_size()) : 8,
+                             lengths.has_value() ? static_cast<int>(lengths->element_size()) : 8, rep, static_cast<float>(repetition_all), pres,
+                             static_cast<float>(presence_all), freq, static_cast<float>(frequency_all), biased ? bias_ids->const_data_ptr() : nullptr,
+                             biased ? bias_values->const_data_ptr<float>() : nullptr, biased ? bias_ids->size(-1) : 0, ids_stride, values_stride,
+                             biased ? static_cast<int>(bias_ids->element_size()) : 8,
+                             allowed.has_value() ? reinterpret_cast<const uint32_t*>(allowed->const_data_ptr<int32_t>()) : nullptr, allowed_stride,
+                             stream_of(logits)),
+             "logit_rules");
+}
+Tensor rules_cuda(const Tensor& logits, const MaybeTensor& history, const MaybeTensor& lengths, const MaybeTensor& repetition, double repetition_all,
+                  const MaybeTensor& presence, double presence_all, const MaybeTensor& frequency, double frequency_all, const MaybeTensor& bias_ids,
+                  const MaybeTensor& bias_values, const MaybeTensor& allowed) {
+    const c10::cuda::CUDAGuard guard(logits.device());
+    Tensor out = at::empty(logits.sizes(), logits.options());
+    rules_into(logits, history, lengths, repetition, repetition_all, presence, presence_all, frequency, frequency_all, bias_ids, bias_values, allowed, out);
+    return out;
+}
+void rules_out_cuda(const Tensor& logits, const MaybeTensor& history, const MaybeTensor& lengths, const MaybeTensor& repetition, double repetition_all,
+                    const MaybeTensor& presence, double presence_all, const MaybeTensor& frequency, double frequency_all, const MaybeTensor& bias_ids,
+                    const MaybeTensor& bias_values, const MaybeTensor& allowed, Tensor& out) {
+    at::assert_no_internal_overlap(out);
+    at::assert_no_partial_overlap(out, logits);   // logits themselves, or memory of its own
+    for (const MaybeTensor* t : {&history, &lengths, &repetition, &presence, &frequency, &bias_ids, &bias_values, &allowed})
+        if (t->has_value()) at::assert_no_overlap(out, **t);
+    rules_into(logits, history, lengths, repetition, repetition_all, presence, presence_all, frequency, frequency_all, bias_ids, bias_values, allowed, out);
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(torch_ggml_ops_b200, m) {
+    m.def("moe_router(Tensor logits, int top_k, int scoring, bool normalize, Tensor? token_mask) -> (Tensor, Tensor)");
+    m.def("moe_router_grad(Tensor grad, Tensor logits, Tensor expert_ids, Tensor weights, int scoring, bool normalize) -> Tensor");
+    m.def("moe_balance_loss(Tensor logits, Tensor expert_ids, int scoring) -> (Tensor, Tensor, Tensor)");
+    m.def("moe_balance_grad(Tensor grad, Tensor logits, Tensor expert_ids, Tensor coef, int scoring) -> Tensor");
+    m.def("moe_dispatch(Tensor input, Tensor expert_ids, int num_experts) -> (Tensor, Tensor, Tensor, Tensor)");
+    m.def("moe_combine(Tensor rows, Tensor row_of_pair, Tensor? weights) -> Tensor");
+    m.def("moe_combine_grad(Tensor grad, Tensor rows, Tensor row_of_pair, Tensor? weights, bool need_rows, bool need_weights) -> (Tensor, Tensor)");
+    m.def(
+        "logit_rules(Tensor logits, Tensor? history, Tensor? history_lengths, Tensor? repetition, float repetition_all, Tensor? presence, "
+        "float presence_all, Tensor? frequency, float frequency_all, Tensor? bias_ids, Tensor? bias_values, Tensor? allowed) -> Tensor");
+    m.def(
+        "logit_rules_out(Tensor logits, Tensor? history, Tensor? history_lengths, Tensor? repetition, float repetition_all, Tensor? presence, "
+        "float presence_all, Tensor? frequency, float frequency_all, Tensor? bias_ids, Tensor? bias_values, Tensor? allowed, Tensor(a!) out) -> ()");
+}
+TORCH_LIBRARY_IMPL(torch_ggml_ops_b200, CUDA, m) {
+    m.impl("moe_router", &router_cuda);
+    m.impl("moe_router_grad", &router_grad_cuda);
+    m.impl("moe_balance_loss", &balance_cuda);
+    m.impl("moe_balance_grad", &balance_grad_cuda);
+    m.impl("moe_dispatch", &dispatch_cuda);
+    m.impl("moe_combine", &combine_cuda);
+    m.impl("moe_combine_grad", &combine_grad_cuda);
+    m.impl("logit_rules", &rules_cuda);
+    m.impl("logit_rules_out", &rules_out_cuda);
+}
+TORCH_LIBRARY_IMPL(torch_ggml_ops_b200, Autograd, m) {
+    m.impl("moe_router", &router_autograd);
+    m.impl("moe_router_grad", &router_grad_autograd);
+    m.impl("moe_balance_loss", &balance_autograd);
+    m.impl("moe_balance_grad", &balance_grad_autograd);
+    m.impl("moe_dispatch", &dispatch_autograd);
+    m.impl("moe_combine", &combine_autograd);
+    m.impl("moe_combine_grad", &combine_grad_autograd);
+}

@@ -31,6 +31,17 @@ SIGNATURES = {
     "tgo_lm_head_loss_workspace_bytes": (_i64, [_i64, _i64, _i64, _i32, _i64]),
     "tgo_lm_head_loss": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i32, _i64, ctypes.c_float, _vp, _vp, _vp, _i64, _vp]),
     "tgo_lm_head_loss_f32": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i32, _i64, ctypes.c_float, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "tgo_moe_router": (_i32, [_vp, _i32, _i64, _i64, _i64, _i64, _i32, _i32, _vp, _vp, _vp, _vp]),
+    "tgo_moe_router_grad": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _i32, _i32, _vp, _vp]),
+    "tgo_moe_balance_workspace_bytes": (_i64, [_i64, _i64]),
+    "tgo_moe_balance_loss": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "tgo_moe_balance_grad": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _i32, _vp, _vp, _vp, _vp]),
+    "tgo_moe_dispatch_workspace_bytes": (_i64, [_i64, _i64]),
+    "tgo_moe_dispatch": (_i32, [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "tgo_moe_combine": (_i32, [_vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
+    "tgo_moe_combine_grad": (_i32, [_vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp]),
+    "tgo_logit_rules": (_i32, [_vp, _vp, _i32, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i32, _i32, _vp, ctypes.c_float, _vp,
+                               ctypes.c_float, _vp, ctypes.c_float, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _i64, _vp]),
     "tgo_grouped_workspace_bytes": (_i64, [_i64, _i64]),
     "tgo_build_tiles": (_i32, [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp]),
     "tgo_grouped_fwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i32, _vp, _i64, _vp]),
