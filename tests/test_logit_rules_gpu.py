@@ -141,6 +141,32 @@ def test_the_same_token_again_and_again(cuda):
     c["bias_ids"][:, ::3] = 3999
     got = check(c)
     assert torch.equal(got, call(c))
+    # sums that are zero in between, tokens that history names too, more entries than tokens
+    c = {"logits": torch.randn(2, 40, generator=torch.Generator().manual_seed(2)), "history": torch.arange(0, 40, 3).repeat(2, 9), "repetition": 1.5,
+         "frequency": 0.25, "bias_ids": torch.arange(40).repeat(2, 64), "bias_values": torch.tensor([1.0, -1.0, 2.0, -2.0]).repeat_interleave(40).repeat(2, 16)}
+    c["bias_values"][1, 7::120] = 3.0
+    check(c)
+    for n in (1, 33, 65, 97):
+        d = dict(c, bias_ids=torch.full((2, n), 9), bias_values=torch.tensor([1.0 if j // 32 % 2 == 0 else -1.0 for j in range(n)]).repeat(2, 1))
+        check(d)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab,n_history,n_bias,mask", [(3, 30011, 8150, 42, True), (3, 30011, 8150, 43, False), (2, 100003, 9000, 300, True),
+                                                              (1, 70000, 70000, 0, True), (1, 3000, 66000, 3000, False), (2, 5000, 3, 9000, True)])
+def test_long_histories_and_lists(cuda, dtype, rows, vocab, n_history, n_bias, mask):
+    """Either table of the named tokens, with counts of 16 and 32 bits, in one block and in several."""
+    import torch_ggml_ops_b200 as tgo
+
+    c = case(rows, vocab, n_history, n_bias, mask, dtype)
+    got = check(c)
+    d = {k: v.cuda() for k, v in c.items()}
+    args = dict(history=d["history"], history_lengths=d["lengths"], repetition_penalty=d["repetition"], presence_penalty=d["presence"],
+                frequency_penalty=d["frequency"], bias_ids=d.get("bias_ids"), bias_values=d.get("bias_values"), allowed=d.get("allowed"))
+    for _ in range(3):
+        x = d["logits"].clone()
+        tgo.logit_rules(x, out=x, **args)
+        assert torch.equal(x, got) and torch.equal(tgo.logit_rules(d["logits"], **args), got)
 
 
 def test_a_large_vocabulary_and_many_rows(cuda):

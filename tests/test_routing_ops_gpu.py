@@ -59,6 +59,19 @@ def test_router_of_equal_scores_takes_the_lower_expert(cuda, dtype, scoring, nor
     check_router(y, 12, scoring, normalize)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("experts,k", [(8, 8), (40, 12), (64, 20), (128, 32), (100, 9), (256, 32), (512, 32), (1024, 32), (777, 17)])
+def test_router_of_sorted_scores(cuda, dtype, experts, k):
+    """The best all lie together, so that one lane of a warp holds many of them, or all that it has."""
+    x = torch.empty(5, experts)
+    ramp = torch.arange(experts) / 8.0
+    x[0], x[1], x[2], x[3] = ramp, -ramp, ramp - 7, (ramp - experts / 16).abs()
+    x[4] = torch.where(torch.arange(experts) % 32 < 4, 50 + ramp / 64, ramp / 64)
+    check_router(x.to(dtype), k, "softmax", True)
+    x[:, ::2] = -math.inf
+    check_router(x.to(dtype), k, "softmax", False)
+
+
 def test_router_of_nearly_equal_scores(cuda):
     """fp32 scores that differ in their last bits only, in every order."""
     base = torch.tensor([1.0, -1.0, 3.1, 1e-30, -1e-30, 77.0, 2.0 ** -130])

@@ -5,9 +5,10 @@
 //   x = -inf where the grammar's mask has no bit for the token
 // in fp32, each operation rounded once, then one rounding to the output's type.
 //
-// One block per slice of a row's vocabulary: it counts the history's tokens that fall into the slice and
-// adds up the biases in shared memory, then passes over the slice once.  So a step is one launch, with no
-// table of counts in memory; every block reads the whole history of its row (from L2).
+// One block per slice of a row's vocabulary: it brings the slice's logits to shared memory, counts the history's
+// tokens that fall into the slice meanwhile, amends the logits of the tokens that history or biases name and
+// writes the slice out under the mask.  One launch, no table of counts in memory; every slice reads all of its row's
+// history (from L2).
 #include "../../include/tgo_mmq.h"
 
 #include <atomic>
@@ -35,14 +36,51 @@ struct RulesArgs {
     int64_t n_bias, bias_ids_stride, bias_values_stride;
     const uint32_t* allowed;   // null: every token
     int64_t allowed_stride;
-    int slice, slices;
+    int slice, slices;   // tokens of a block, blocks of a row
     bool history_wide, lengths_wide, bias_wide, vectors, in_place;
 };
 
 __device__ __forceinline__ int64_t id_at(const void* p, bool wide, int64_t i) {
     return wide ? static_cast<const int64_t*>(p)[i] : static_cast<int64_t>(static_cast<const int32_t*>(p)[i]);
 }
+// An id's distance from token lo; kNone unless it is one of the span tokens from there on
+constexpr uint32_t kNone = 0xFFFFFFFFu;
+__device__ __forceinline__ uint32_t distance(uint32_t id, uint32_t lo, uint32_t span) { return id - lo < span ? id - lo : kNone; }
+__device__ __forceinline__ uint32_t distance(uint2 id, uint32_t lo, uint32_t span) { return id.y == 0 && id.x - lo < span ? id.x - lo : kNone; }
 
+// f(d[kAhead]) for the distances of ids, by the block's whole warps, where a lane has one: several ids are
+// under way per thread, so that the loop waits for L2 once in so many.
+constexpr int kAhead = 8;
+template <typename Id, typename F>
+__device__ __forceinline__ void each_id(const Id* __restrict__ ids, int64_t n, uint32_t lo, uint32_t span, F f) {
+    const int lane = threadIdx.x & 31;
+    ids += threadIdx.x;
+    for (int64_t left = n - (threadIdx.x - lane); left > 0; left -= kRulesThreads * kAhead, ids += kRulesThreads * kAhead) {
+        Id id[kAhead];
+        uint32_t d[kAhead];
+        bool any = false;
+        if (left >= kRulesThreads * (kAhead - 1) + 32) {
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) id[u] = ids[u * kRulesThreads];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                d[u] = distance(id[u], lo, span);
+                any |= d[u] != kNone;
+            }
+        } else {
+            const int mine = static_cast<int>(left) - lane;
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+                if (u * kRulesThreads < mine) id[u] = ids[u * kRulesThreads];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                d[u] = u * kRulesThreads < mine ? distance(id[u], lo, span) : kNone;
+                any |= d[u] != kNone;
+            }
+        }
+        if (__any_sync(kAllLanes, any)) f(d);
+    }
+}
 struct Penalty {
     float repetition, presence, frequency;
 };
@@ -51,156 +89,270 @@ __device__ __forceinline__ float penalised(float x, uint32_t count, const Penalt
     return __fsub_rn(x, __fadd_rn(__fmul_rn(static_cast<float>(count), p.frequency), p.presence));
 }
 
+// What a block works on, from the row's first 16-byte boundary on in vectors
 template <typename T>
-__global__ void __launch_bounds__(kRulesThreads) logit_rules_kernel(RulesArgs a) {
-    extern __shared__ uint4 smem[];
-    constexpr int VEC = 16 / static_cast<int>(sizeof(T));
-    const int64_t row = blockIdx.x / static_cast<unsigned>(a.slices);
-    const int part = static_cast<int>(blockIdx.x - row * a.slices);
-    const T* in = static_cast<const T*>(a.logits) + row * a.in_stride;
-    T* out = static_cast<T*>(a.out) + row * a.out_stride;
-    // elements in front of the row's first 16-byte boundary; they go with the first slice
-    int head = a.vectors ? static_cast<int>((16 - reinterpret_cast<uintptr_t>(in) % 16) % 16 / sizeof(T)) : 0;
-    if (head > a.vocab) head = static_cast<int>(a.vocab);
-    const int64_t base = head + static_cast<int64_t>(part) * a.slice;   // what shared memory calls token kRulesPad
-    const int64_t lo = part == 0 ? 0 : base;
-    const int64_t hi = base + a.slice < a.vocab ? base + a.slice : a.vocab;
-    if (lo >= hi) return;
-
-    const bool counting = a.history != nullptr, biased = a.bias_ids != nullptr;
-    uint32_t* count = reinterpret_cast<uint32_t*>(smem);
-    float* bias = reinterpret_cast<float*>(count + (counting ? a.slice + kRulesPad : 0));
-    Penalty pen = {1.0f, 0.0f, 0.0f};
-    if (counting || biased) {
-        const int words = (a.slice + kRulesPad) * ((counting ? 1 : 0) + (biased ? 1 : 0));
-        for (int i = threadIdx.x; i < words; i += kRulesThreads) count[i] = 0;
-        __syncthreads();
+struct Slice {
+    static constexpr int VEC = 16 / static_cast<int>(sizeof(T));
+    static constexpr uint32_t kAll = (1u << VEC) - 1u;
+    int64_t row;
+    int part;
+    const T* in;
+    T* out;
+    int64_t base, lo, hi;    // tokens lo..hi-1; base: the first at a boundary of `in` (lo is in front of it in a row's first slice)
+    const uint32_t* words;   // the row's mask
+    __device__ __forceinline__ explicit Slice(const RulesArgs& a) {
+        row = blockIdx.x / static_cast<unsigned>(a.slices);
+        part = static_cast<int>(blockIdx.x - row * a.slices);
+        in = static_cast<const T*>(a.logits) + row * a.in_stride;
+        out = static_cast<T*>(a.out) + row * a.out_stride;
+        int head = static_cast<int>((16 - reinterpret_cast<uintptr_t>(in) % 16) % 16 / sizeof(T));
+        if (head > a.vocab) head = static_cast<int>(a.vocab);
+        base = head + static_cast<int64_t>(part) * a.slice;
+        lo = part == 0 ? 0 : base;
+        hi = base + a.slice < a.vocab ? base + a.slice : a.vocab;
+        words = a.allowed != nullptr ? a.allowed + row * a.allowed_stride : nullptr;
     }
+    __device__ __forceinline__ int vecs() const { return hi > base ? static_cast<int>((hi - base) / VEC) : 0; }
+    // f(token) for the elements that are in no vector, up to VEC - 1 on either side
+    template <typename F>
+    __device__ __forceinline__ void edges(F f) const {
+        if (lo + threadIdx.x < base && lo + threadIdx.x < hi) f(lo + threadIdx.x);
+        const int64_t rest = base + static_cast<int64_t>(vecs()) * VEC;
+        if (rest + threadIdx.x < hi) f(rest + threadIdx.x);
+    }
+    // The slice under its mask to memory, several vectors of each thread under way: x(v) is vector v, same(v) whether it may stay as
+    // it is in memory, one(token) an element.
+    template <typename X, typename S, typename O>
+    __device__ __forceinline__ void finish(const RulesArgs& a, X x, S same, O one) const {
+        auto put = [&](int64_t t) { out[t] = words == nullptr || (words[t >> 5] >> (t & 31) & 1u) != 0 ? one(t) : from_f32<T>(-INFINITY); };
+        if (!a.vectors) {
+            for (int64_t t = lo + threadIdx.x; t < hi; t += kRulesThreads) put(t);
+            return;
+        }
+        edges(put);
+        const int n = vecs();
+        constexpr int kDeep = 4;
+        for (int v0 = threadIdx.x; v0 < n; v0 += kRulesThreads * kDeep) {
+            Pack<T, VEC> p[kDeep];
+            uint32_t bits[kDeep], w[2][kDeep];
+            bool skip[kDeep];
+#pragma unroll
+            for (int u = 0; u < kDeep; ++u) {
+                const int64_t t = base + static_cast<int64_t>(v0 + u * kRulesThreads) * VEC;
+                w[0][u] = w[1][u] = 0xFFFFFFFFu;
+                if (words != nullptr && v0 + u * kRulesThreads < n) w[0][u] = words[t >> 5], w[1][u] = words[(t + VEC - 1) >> 5];
+            }
+#pragma unroll
+            for (int u = 0; u < kDeep; ++u) {
+                const int v = v0 + u * kRulesThreads;
+                bits[u] = __funnelshift_r(w[0][u], w[1][u], static_cast<uint32_t>((base + static_cast<int64_t>(v) * VEC) & 31)) & kAll;
+                skip[u] = v >= n || (bits[u] == kAll && same(v));
+                if (!skip[u] && bits[u] != 0) p[u] = x(v);
+            }
+#pragma unroll
+            for (int u = 0; u < kDeep; ++u) {
+                if (skip[u]) continue;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    if ((bits[u] >> j & 1u) == 0) p[u].v[j] = from_f32<T>(-INFINITY);
+                *reinterpret_cast<Pack<T, VEC>*>(out + base + static_cast<int64_t>(v0 + u * kRulesThreads) * VEC) = p[u];
+            }
+        }
+    }
+};
+
+// the mask alone
+template <typename T>
+__global__ void __launch_bounds__(kRulesThreads, 4) logit_mask_kernel(RulesArgs a) {
+    const Slice<T> s(a);
+    using Vec = Pack<T, Slice<T>::VEC>;
+    s.finish(
+        a, [&](int v) { return *reinterpret_cast<const Vec*>(s.in + s.base + static_cast<int64_t>(v) * Slice<T>::VEC); }, [&](int) { return a.in_place; },
+        [&](int64_t t) { return s.in[t]; });
+}
+
+// C: type of a count; 16 bits where no history is longer than they count.  Shared memory: the slice's logits, its
+// counts, its biases, each from token base - kRulesPad on; then the tokens that history or biases name, each once, so that the
+// arithmetic runs on 32 of them at a time however thinly they lie.
+template <typename T, typename C>
+__global__ void __launch_bounds__(kRulesThreads, 4) logit_rules_kernel(RulesArgs a) {
+    extern __shared__ uint4 smem[];
+    __shared__ int n_named;
+    const Slice<T> s(a);
+    constexpr int VEC = Slice<T>::VEC;
+    const int tokens = a.slice + kRulesPad, lane = threadIdx.x & 31;
+    const bool counting = a.history != nullptr, biased = a.bias_ids != nullptr;
+    T* x = reinterpret_cast<T*>(smem);
+    C* count = reinterpret_cast<C*>(x + tokens);
+    float* bias = reinterpret_cast<float*>(counting ? count + tokens : count);   // +0 until a bias has named the token (a sum of 0 is kept as -0)
+    uint16_t* named = reinterpret_cast<uint16_t*>(biased ? bias + tokens : bias);
+
+    // the logits on their way while the tables are made
+    for (int v = threadIdx.x; v < s.vecs(); v += kRulesThreads)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<unsigned>(__cvta_generic_to_shared(x + kRulesPad + v * VEC))),
+                     "l"(s.in + s.base + static_cast<int64_t>(v) * VEC)
+                     : "memory");
+    Penalty pen = {1.0f, 0.0f, 0.0f};
+    int64_t n = 0;   // ids of the row's history
     if (counting) {
-        pen.repetition = a.repetition != nullptr ? a.repetition[row] : a.repetition_all;
-        pen.presence = a.presence != nullptr ? a.presence[row] : a.presence_all;
-        pen.frequency = a.frequency != nullptr ? a.frequency[row] : a.frequency_all;
-        int64_t n = a.history_len;
+        n = a.history_len;
         if (a.lengths != nullptr) {
-            const int64_t own = id_at(a.lengths, a.lengths_wide, row);
+            const int64_t own = id_at(a.lengths, a.lengths_wide, s.row);
             n = own < n ? own : n;
         }
-        for (int64_t i = threadIdx.x; i < n; i += kRulesThreads) {
-            const int64_t t = id_at(a.history, a.history_wide, row * a.history_stride + i);
-            if (t >= lo && t < hi) atomicAdd(&count[t - base + kRulesPad], 1u);
-        }
+        pen.repetition = a.repetition != nullptr ? a.repetition[s.row] : a.repetition_all;
+        pen.presence = a.presence != nullptr ? a.presence[s.row] : a.presence_all;
+        pen.frequency = a.frequency != nullptr ? a.frequency[s.row] : a.frequency_all;
     }
+    s.edges([&](int64_t t) { x[t - s.base + kRulesPad] = s.in[t]; });
+    {
+        uint4* table = reinterpret_cast<uint4*>(count);
+        const int chunks = tokens * static_cast<int>((counting ? sizeof(C) : 0) + (biased ? 4 : 0)) / 16;
+        for (int i = threadIdx.x; i < chunks; i += kRulesThreads) table[i] = make_uint4(0, 0, 0, 0);
+        if (threadIdx.x == 0) n_named = 0;
+        __syncthreads();
+    }
+    const uint32_t span = s.hi > s.lo ? static_cast<uint32_t>(s.hi - s.lo) : 0u;
+    const int first = static_cast<int>(s.lo - s.base) + kRulesPad;
+    // Counts tokens and lists those that are counted for the first time: a warp joins what its threads give to the list at once.
+    auto add = [&](const uint32_t(&d)[kAhead]) {
+        uint32_t before[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            before[u] = 1;
+            if (d[u] == kNone) continue;
+            const unsigned i = d[u] + first;
+            unsigned* table = reinterpret_cast<unsigned*>(count);
+            if (sizeof(C) == 4) before[u] = atomicAdd(table + i, 1u);
+            else before[u] = atomicAdd(table + i / 2, i % 2 ? 0x10000u : 1u) >> (i % 2 * 16) & 0xFFFFu;
+        }
+        int mine = 0;
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) mine += before[u] == 0;
+        if (!__any_sync(kAllLanes, mine != 0)) return;
+        int upto = mine;
+#pragma unroll
+        for (int l = 1; l < 32; l <<= 1) {
+            const int o = __shfl_up_sync(kAllLanes, upto, l);
+            if (lane >= l) upto += o;
+        }
+        int at = 0;
+        if (lane == 31) at = atomicAdd(&n_named, upto);
+        at = __shfl_sync(kAllLanes, at, 31) + upto - mine;
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (before[u] == 0) named[at++] = static_cast<uint16_t>(d[u] + first);
+    };
+    if (counting) {
+        const int64_t at = s.row * a.history_stride;
+        if (a.history_wide) each_id(static_cast<const uint2*>(a.history) + at, n, static_cast<uint32_t>(s.lo), span, add);
+        else each_id(static_cast<const uint32_t*>(a.history) + at, n, static_cast<uint32_t>(s.lo), span, add);
+    }
+    if (biased) __syncthreads();
     if (biased && threadIdx.x < 32) {
         // one warp, 32 entries at a time, each token's in the order of the list: the same sum every time
-        const int lane = threadIdx.x;
         for (int64_t j0 = 0; j0 < a.n_bias; j0 += 32) {
             int64_t t = -1;
             float v = 0.0f;
             if (j0 + lane < a.n_bias) {
-                t = id_at(a.bias_ids, a.bias_wide, row * a.bias_ids_stride + j0 + lane);
-                if (t < lo || t >= hi) t = -1;
-                else v = a.bias_values[row * a.bias_values_stride + j0 + lane];
+                t = id_at(a.bias_ids, a.bias_wide, s.row * a.bias_ids_stride + j0 + lane);
+                if (t < s.lo || t >= s.hi) t = -1;
+                else v = a.bias_values[s.row * a.bias_values_stride + j0 + lane];
             }
+            if (!__any_sync(kAllLanes, t >= 0)) continue;
             const unsigned same = __match_any_sync(kAllLanes, t);
-            const bool first = (same & ((1u << lane) - 1u)) == 0;
-            float sum = first && t >= 0 ? bias[t - base + kRulesPad] : 0.0f;
-            for (int s = 0; s < 32; ++s) {
-                const float o = __shfl_sync(kAllLanes, v, s);
-                if (same >> s & 1u) sum = __fadd_rn(sum, o);
+            const bool leads = t >= 0 && (same & ((1u << lane) - 1u)) == 0;
+            const int i = static_cast<int>(t - s.base) + kRulesPad;
+            const float old = leads ? bias[i] : 0.0f;
+            float sum = old;
+            for (int l = 0; l < 32; ++l) {
+                const float o = __shfl_sync(kAllLanes, v, l);
+                if (same >> l & 1u) sum = __fadd_rn(sum, o);
             }
-            if (first && t >= 0) bias[t - base + kRulesPad] = sum;
+            if (leads) bias[i] = sum == 0.0f ? -0.0f : sum;
+            const bool fresh = leads && __float_as_uint(old) == 0u && !(counting && count[i] != 0);
+            const unsigned who = __ballot_sync(kAllLanes, fresh);
+            if (fresh) named[n_named + __popc(who & ((1u << lane) - 1u))] = static_cast<uint16_t>(i);
+            __syncwarp();
+            if (lane == 0) n_named += __popc(who);
             __syncwarp();
         }
     }
-    if (counting || biased) __syncthreads();
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
 
-    const uint32_t* words = a.allowed != nullptr ? a.allowed + row * a.allowed_stride : nullptr;
-    auto one = [&](int64_t t) {
-        const bool on = words == nullptr || (words[t >> 5] >> (t & 31) & 1u) != 0;
-        const int i = static_cast<int>(t - base) + kRulesPad;
-        const uint32_t c = counting ? count[i] : 0u;
+    for (int j = threadIdx.x; j < n_named; j += kRulesThreads) {
+        const int i = named[j];
         const float b = biased ? bias[i] : 0.0f;
-        if (!on) {
-            out[t] = from_f32<T>(-INFINITY);
-        } else if (c != 0 || b != 0.0f) {
-            float x = to_f32(in[t]);
-            if (b != 0.0f) x = __fadd_rn(x, b);
-            if (c != 0) x = penalised(x, c, pen);
-            out[t] = from_f32<T>(x);
-        } else if (!a.in_place) {
-            out[t] = in[t];
-        }
-    };
-    if (!a.vectors) {
-        for (int64_t t = lo + threadIdx.x; t < hi; t += kRulesThreads) one(t);
-        return;
+        const uint32_t c = counting ? count[i] : 0u;
+        if (c == 0 && b == 0.0f) continue;
+        float f = to_f32(x[i]);
+        if (b != 0.0f) f = __fadd_rn(f, b);
+        if (c != 0) f = penalised(f, c, pen);
+        x[i] = from_f32<T>(f);
     }
-    if (lo + threadIdx.x < base) one(lo + threadIdx.x);   // the head
-    const int vecs = static_cast<int>((hi - base) / VEC);
-    for (int v = threadIdx.x; v < vecs; v += kRulesThreads) {
-        const int64_t t = base + static_cast<int64_t>(v) * VEC;
-        uint32_t on = (1u << VEC) - 1u;
-        if (words != nullptr) {
-            const uint32_t w0 = words[t >> 5], w1 = words[(t + VEC - 1) >> 5];
-            on &= __funnelshift_r(w0, w1, static_cast<uint32_t>(t & 31));
-        }
-        uint32_t changed = 0;
-        uint32_t c[VEC];
-        float b[VEC];
-        const int i = v * VEC + kRulesPad;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) c[j] = 0, b[j] = 0.0f;
-        if (counting) {
-#pragma unroll
-            for (int j = 0; j < VEC; j += 4) {
-                const uint4 q = *reinterpret_cast<const uint4*>(count + i + j);
-                c[j] = q.x, c[j + 1] = q.y, c[j + 2] = q.z, c[j + 3] = q.w;
-            }
-        }
-        if (biased) {
-#pragma unroll
-            for (int j = 0; j < VEC; j += 4) {
-                const float4 q = *reinterpret_cast<const float4*>(bias + i + j);
-                b[j] = q.x, b[j + 1] = q.y, b[j + 2] = q.z, b[j + 3] = q.w;
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) changed |= (c[j] != 0 || b[j] != 0.0f ? 1u : 0u) << j;
-        changed &= on;
-        if (a.in_place && changed == 0 && on == (1u << VEC) - 1u) continue;
-        Pack<T, VEC> x = {};
-        if (on != 0) x = *reinterpret_cast<const Pack<T, VEC>*>(in + t);
-        if (changed != 0) {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                if ((changed >> j & 1u) == 0) continue;
-                float f = to_f32(x.v[j]);
-                if (b[j] != 0.0f) f = __fadd_rn(f, b[j]);
-                if (c[j] != 0) f = penalised(f, c[j], pen);
-                x.v[j] = from_f32<T>(f);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < VEC; ++j)
-            if ((on >> j & 1u) == 0) x.v[j] = from_f32<T>(-INFINITY);
-        *reinterpret_cast<Pack<T, VEC>*>(out + t) = x;
-    }
-    const int64_t rest = base + static_cast<int64_t>(vecs) * VEC;
-    if (rest + threadIdx.x < hi) one(rest + threadIdx.x);
+    __syncthreads();
+    using Vec = Pack<T, VEC>;
+    s.finish(
+        a, [&](int v) { return *reinterpret_cast<const Vec*>(x + kRulesPad + v * VEC); },
+        [&](int v) {
+            if (!a.in_place) return false;
+            bool none = true;
+            for (int j = kRulesPad + v * VEC; j < kRulesPad + (v + 1) * VEC; ++j) none &= !(counting && count[j] != 0) && !(biased && bias[j] != 0.0f);
+            return none;
+        },
+        [&](int64_t t) { return x[t - s.base + kRulesPad]; });
 }
 
-template <typename T>
-static int launch_rules(const RulesArgs& a, size_t smem, cudaStream_t st) {
+// ------------------------------------------------------------------ launches
+constexpr int64_t kRulesMemory = 55 * 1024;   // shared memory of a block: four of them on an SM
+
+template <typename T, typename C>
+static int launch_slices(const RulesArgs& a, size_t smem, cudaStream_t st) {
     static std::atomic<bool> ready[64];   // a kernel may use more than 48 KB only after a call per device has said so
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return route_fail(TGO_E_CUDA, "cudaGetDevice failed");
     if (dev >= 64 || !ready[dev].load(std::memory_order_relaxed)) {
-        if (cudaFuncSetAttribute(logit_rules_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) != cudaSuccess)
+        if (cudaFuncSetAttribute(logit_rules_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kRulesMemory)) != cudaSuccess)
             return route_fail(TGO_E_CUDA, "cudaFuncSetAttribute failed");
         if (dev < 64) ready[dev].store(true, std::memory_order_relaxed);
     }
-    logit_rules_kernel<T><<<static_cast<unsigned>(a.rows * a.slices), kRulesThreads, smem, st>>>(a);
+    logit_rules_kernel<T, C><<<static_cast<unsigned>(a.rows * a.slices), kRulesThreads, smem, st>>>(a);
     return cudaGetLastError() == cudaSuccess ? TGO_OK : route_fail(TGO_E_CUDA, "logit_rules_kernel launch failed");
+}
+
+template <typename T>
+static int launch_rules(RulesArgs& a, int64_t id_bytes, cudaStream_t st) {
+    const bool tables = a.history != nullptr || a.bias_ids != nullptr, narrow = a.history_len <= UINT16_MAX;
+    const int64_t token_bytes = static_cast<int64_t>(sizeof(T)) + (a.history != nullptr ? (narrow ? 2 : 4) : 0) + (a.bias_ids != nullptr ? 4 : 0);
+    // the list of named tokens is as long as history and biases together, or as the slice
+    const int64_t all_names = a.history_len + a.n_bias;
+    int64_t most = 16384;
+    if (tables) {
+        const int64_t long_list = kRulesMemory / (token_bytes + 2), short_list = all_names < kRulesMemory ? (kRulesMemory - 2 * all_names) / token_bytes : 0;
+        most = ((long_list > short_list ? long_list : short_list) - kRulesPad - 1) / 128 * 128;
+    }
+    // some four blocks per SM, no slice shorter than 1024 tokens, none longer than its shared memory takes
+    int64_t slices = (148 * 4 + a.rows - 1) / a.rows;
+    if (slices > (a.vocab + 1023) / 1024) slices = (a.vocab + 1023) / 1024;
+    if (a.history != nullptr) {
+        // Of a long history that every slice reads: so few slices that it is no more than twice what they read and write else, down to a
+        // block per SM (us with / without, bf16: 4 rows of 65535 ids 27.9 / 39.3, 16 rows 38.4 / 53.0; 16 rows of 4096 ids 14.3 / 14.4).
+        const int64_t fair = 4 * a.vocab * static_cast<int64_t>(sizeof(T)) / (a.history_len * id_bytes), fewest = (148 + a.rows - 1) / a.rows;
+        if (slices > fair) slices = fair > fewest ? fair : fewest < slices ? fewest : slices;
+    }
+    if (slices < (a.vocab + most - 1) / most) slices = (a.vocab + most - 1) / most;
+    if (a.rows > INT32_MAX / slices) return route_fail(TGO_E_ARG, "too many logits");
+    a.slices = static_cast<int>(slices);
+    a.slice = static_cast<int>(((a.vocab + slices - 1) / slices + 127) / 128 * 128);
+    if (!tables) {
+        if (a.in_place && a.allowed == nullptr) return TGO_OK;
+        logit_mask_kernel<T><<<static_cast<unsigned>(a.rows * slices), kRulesThreads, 0, st>>>(a);
+        return cudaGetLastError() == cudaSuccess ? TGO_OK : route_fail(TGO_E_CUDA, "logit_mask_kernel launch failed");
+    }
+    const int64_t names = all_names < a.slice + kRulesPad ? all_names : a.slice + kRulesPad;
+    const size_t smem = static_cast<size_t>(token_bytes) * (a.slice + kRulesPad) + static_cast<size_t>(names) * 2;
+    return narrow ? launch_slices<T, uint16_t>(a, smem, st) : launch_slices<T, uint32_t>(a, smem, st);
 }
 
 }  // namespace tgo
@@ -228,28 +380,18 @@ extern "C" int tgo_logit_rules(const void* logits, void* out, int dtype, int64_t
     if (i % size != 0 || o % size != 0) return route_fail(TGO_E_ARG, "logits are not aligned to their type");
     RulesArgs a = {};
     a.logits = logits, a.out = out, a.rows = rows, a.vocab = vocab, a.in_stride = in_stride, a.out_stride = out_stride;
-    if (history_len > 0) a.history = history, a.lengths = lengths, a.history_len = history_len, a.history_stride = history_stride;
+    if (history != nullptr && history_len > 0) a.history = history, a.lengths = lengths, a.history_len = history_len, a.history_stride = history_stride;
     a.history_wide = history_id_bytes == 8, a.lengths_wide = length_bytes == 8;
     a.repetition = repetition, a.presence = presence, a.frequency = frequency;
     a.repetition_all = repetition_all, a.presence_all = presence_all, a.frequency_all = frequency_all;
-    if (n_bias > 0) a.bias_ids = bias_ids, a.bias_values = bias_values, a.n_bias = n_bias;
+    if (bias_ids != nullptr && n_bias > 0) a.bias_ids = bias_ids, a.bias_values = bias_values, a.n_bias = n_bias;
     a.bias_ids_stride = bias_ids_stride, a.bias_values_stride = bias_values_stride, a.bias_wide = bias_id_bytes == 8;
     a.allowed = allowed, a.allowed_stride = allowed_stride;
     a.in_place = logits == out && (rows == 1 || in_stride == out_stride);
     // 16-byte accesses where every row of the result lies to its boundary as the row of logits does
     a.vectors = (i - o) % 16 == 0 && (rows == 1 || (in_stride - out_stride) * size % 16 == 0);
-    const int tables = (a.history != nullptr ? 1 : 0) + (a.bias_ids != nullptr ? 1 : 0);
-    // slices: some four blocks per SM, no shorter than 1024 tokens, at most 64 KB of shared memory each
-    int64_t slices = (148 * 4 + rows - 1) / rows;
-    int64_t slice = (vocab + slices - 1) / slices;
-    const int64_t most = tables == 2 ? 8192 : 16384;
-    slice = slice < 1024 ? 1024 : slice > most ? most : (slice + 127) / 128 * 128;
-    slices = (vocab + slice - 1) / slice;
-    if (rows > INT32_MAX / slices) return route_fail(TGO_E_ARG, "too many logits");
-    a.slice = static_cast<int>(slice), a.slices = static_cast<int>(slices);
-    const size_t smem = static_cast<size_t>(tables) * (slice + kRulesPad) * 4;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == TGO_BF16) return launch_rules<__nv_bfloat16>(a, smem, st);
-    if (dtype == TGO_FP16) return launch_rules<__half>(a, smem, st);
-    return launch_rules<float>(a, smem, st);
+    if (dtype == TGO_BF16) return launch_rules<__nv_bfloat16>(a, history_id_bytes, st);
+    if (dtype == TGO_FP16) return launch_rules<__half>(a, history_id_bytes, st);
+    return launch_rules<float>(a, history_id_bytes, st);
 }

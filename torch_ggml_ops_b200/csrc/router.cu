@@ -39,26 +39,35 @@ struct RowLayout {
     }
 };
 
-// x[v] = the row's scores, -inf beyond the last expert
+// A lane's part of a row as it lies in memory, so that the next row can be under way while one is worked on
 template <typename T, int VPL>
-__device__ __forceinline__ void load_row(const T* __restrict__ row, int experts, bool chunks, int lane, float (&x)[VPL]) {
+struct RawRow {
     using L = RowLayout<T, VPL>;
-    if (chunks) {
+    Pack<T, L::CH> p[VPL / L::CH];
+    __device__ __forceinline__ void load(const T* __restrict__ row, int experts, bool chunks, int lane) {
 #pragma unroll
         for (int c = 0; c < VPL / L::CH; ++c) {
             const int e = L::expert(c * L::CH, lane);
-            Pack<T, L::CH> p;
-            if (e < experts) p = *reinterpret_cast<const Pack<T, L::CH>*>(row + e);
+            if (chunks) {
+                if (e < experts) p[c] = *reinterpret_cast<const Pack<T, L::CH>*>(row + e);
+            } else {
 #pragma unroll
-            for (int j = 0; j < L::CH; ++j) x[c * L::CH + j] = e < experts ? to_f32(p.v[j]) : -INFINITY;
-        }
-    } else {
-#pragma unroll
-        for (int v = 0; v < VPL; ++v) {
-            const int e = L::expert(v, lane);
-            x[v] = e < experts ? to_f32(row[e]) : -INFINITY;
+                for (int j = 0; j < L::CH; ++j)
+                    if (e + j < experts) p[c].v[j] = row[e + j];
+            }
         }
     }
+    // x[v] = the scores, -inf beyond the last expert
+    __device__ __forceinline__ void widen(int experts, int lane, float (&x)[VPL]) const {
+#pragma unroll
+        for (int v = 0; v < VPL; ++v) x[v] = L::expert(v, lane) < experts ? to_f32(p[v / L::CH].v[v % L::CH]) : -INFINITY;
+    }
+};
+template <typename T, int VPL>
+__device__ __forceinline__ void load_row(const T* __restrict__ row, int experts, bool chunks, int lane, float (&x)[VPL]) {
+    RawRow<T, VPL> raw;
+    raw.load(row, experts, chunks, lane);
+    raw.widen(experts, lane, x);
 }
 template <typename T, int VPL>
 __device__ __forceinline__ void store_row(T* __restrict__ row, int experts, bool chunks, int lane, const float (&x)[VPL]) {
@@ -81,6 +90,20 @@ __device__ __forceinline__ void store_row(T* __restrict__ row, int experts, bool
     }
 }
 
+template <typename T, int VPL>
+__device__ __forceinline__ void copy_row(T* __restrict__ row, const T* from, int experts, bool chunks, int lane) {
+    using L = RowLayout<T, VPL>;
+    if (chunks) {
+#pragma unroll
+        for (int c = 0; c < VPL / L::CH; ++c) {
+            const int e = L::expert(c * L::CH, lane);
+            if (e < experts) *reinterpret_cast<Pack<T, L::CH>*>(row + e) = *reinterpret_cast<const Pack<T, L::CH>*>(from + e);
+        }
+    } else {
+        for (int e = lane; e < experts; e += 32) row[e] = from[e];
+    }
+}
+
 __device__ __forceinline__ float log_sigmoid(float x) { return fminf(x, 0.0f) - log1pf(expf(-fabsf(x))); }
 __device__ __forceinline__ float sigmoid_of_minus(float x) {
     const float far = expf(-fabsf(x));
@@ -95,26 +118,33 @@ __device__ __forceinline__ float warp_max(const float (&x)[VPL]) {
     float m = x[0];
 #pragma unroll
     for (int v = 1; v < VPL; ++v) m = fmaxf(m, x[v]);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(kAllLanes, m, d));
+    asm("redux.sync.max.f32 %0, %0, 0xffffffff;" : "+f"(m));
     return m;
 }
 
-// u -> exp(u) / sum of them, 0 everywhere in a row of -inf; a NaN or +inf among them makes all of them NaN
+// exp(d) of a difference d <= 0 for the sums over all experts, in three instructions where expf takes eight: off by
+// 4 U + 1.3 |d| U of itself (U = 2^-24): little where it is large, and where it is small it adds little to a sum;
+// below 2^-126 it is 0.
+__device__ __forceinline__ float exp_below(float d) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * 1.4426950408889634f));
+    return r;
+}
+
+// u -> exp(u - the largest); returns 1 / their sum, 0 for a row of -inf.  With a NaN or +inf in the row the products
+// with it are all NaN.
 template <int VPL>
-__device__ __forceinline__ void shares(float (&u)[VPL]) {
+__device__ __forceinline__ float exponentials(float (&u)[VPL]) {
     float m = warp_max(u);
     if (m == -INFINITY) m = 0.0f;
     float s = 0.0f;
 #pragma unroll
     for (int v = 0; v < VPL; ++v) {
-        u[v] = expf(u[v] - m);
+        u[v] = exp_below(u[v] - m);
         s += u[v];
     }
     s = warp_sum(s);
-    const float inv = s == 0.0f ? 0.0f : 1.0f / s;
-#pragma unroll
-    for (int v = 0; v < VPL; ++v) u[v] *= inv;
+    return s == 0.0f ? 0.0f : 1.0f / s;
 }
 
 struct RouterArgs {
@@ -128,7 +158,7 @@ struct RouterArgs {
 // The top_k largest scores in order, lane s the s-th: (score, expert); of equal scores the lower expert
 // first.  -inf and NaN are never chosen: expert -1 where nothing is left.
 template <typename T, int VPL>
-__device__ __forceinline__ void choose(const float (&x)[VPL], int top_k, int lane, float& score, int& expert) {
+__device__ __noinline__ void choose_exactly(const float (&x)[VPL], int top_k, int lane, float& score, int& expert) {
     using L = RowLayout<T, VPL>;
     uint32_t key[VPL];   // 0: not to be chosen (any more)
 #pragma unroll
@@ -158,44 +188,114 @@ __device__ __forceinline__ void choose(const float (&x)[VPL], int top_k, int lan
     }
 }
 
+// the largest of a lane's keys that is below `last`, one of them; 0 if there is none.  Keys below last wrap around
+// to the largest differences.
+template <int VPL>
+__device__ __forceinline__ uint32_t next_below(const uint32_t (&key)[VPL], uint32_t last) {
+    uint32_t m = key[0] - last;
+#pragma unroll
+    for (int v = 1; v < VPL; ++v) m = max(m, key[v] - last);
+    return m + last < last ? m + last : 0u;
+}
+
+// The same with one reduction per choice and no search for the expert: a key holds the upper 22 bits of a score's
+// order and, below, the expert (the lower expert the larger number), so that no two are equal.  That is all of a
+// 16-bit score.  Of two fp32 scores that agree in the 22 bits the exact comparison decides: a row where such are
+// among the best (1 in 70 of 256 normal scores) goes through choose_exactly.
+// First the best top_k of the lanes' best, in order; lane s holds the s-th.  Scores of the same lanes that belong
+// among them (one or two in a row as a rule) are then put in one by one.
+// bad: the row holds a NaN (its order, like any NaN's after the addition of 0, is above all).
+constexpr uint32_t kExpertBits = 1023;
+template <typename T, int VPL>
+__device__ __forceinline__ void choose(const float (&x)[VPL], const T* __restrict__ row, int top_k, int lane, float& score, int& expert, bool& bad) {
+    using L = RowLayout<T, VPL>;
+    constexpr bool kWide = sizeof(T) == 4;
+    constexpr uint32_t kLeast = 0x00800000u;     // order of the lowest finite fp32 (fp16's and bf16's are no lower): -inf is below
+    constexpr uint32_t kInfinite = 0xFF800000u;  // order of +inf
+    uint32_t key[VPL];
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) key[v] = (order_of(x[v]) & ~kExpertBits) | (kExpertBits - L::expert(v, lane));
+    uint32_t first = key[0];
+#pragma unroll
+    for (int v = 1; v < VPL; ++v) first = max(first, key[v]);
+    uint32_t mine = 0, low = 0, left = first;
+    const int slots = kWide && top_k < 32 ? top_k + 1 : top_k;   // fp32: whether the next one is as large has to be seen
+    for (int s = 0; s < slots; ++s) {
+        low = __reduce_max_sync(kAllLanes, left);
+        if (lane == s) mine = low;
+        if (left == low) left = 0;
+    }
+    bad = __shfl_sync(kAllLanes, mine, 0) > (kInfinite | kExpertBits);
+    if (VPL > 1) {
+        // `low` is the least that is in; a lane whose best is out has nothing that is better
+        uint32_t next = first >= low ? next_below(key, first) : 0u;
+        while (__any_sync(kAllLanes, next > low)) {
+            const uint32_t put = __reduce_max_sync(kAllLanes, next);
+            const uint32_t above = __shfl_up_sync(kAllLanes, mine, 1);
+            mine = max(mine, lane == 0 ? put : min(above, put));
+            low = __shfl_sync(kAllLanes, mine, slots - 1);
+            if (next == put) next = next_below(key, put);
+        }
+    }
+    if (kWide) {
+        // the last of 32 has no slot behind it: whether another one is as large is looked up
+        const uint32_t above = __shfl_up_sync(kAllLanes, mine, 1);
+        bool close = lane > 0 && lane < slots && mine >= kLeast && ((mine ^ above) & ~kExpertBits) == 0;
+        if (top_k == 32) {
+#pragma unroll
+            for (int v = 0; v < VPL; ++v) close |= ((key[v] ^ low) & ~kExpertBits) == 0 && key[v] < low;
+        }
+        if (__any_sync(kAllLanes, close) || bad) {
+            choose_exactly<T, VPL>(x, top_k, lane, score, expert);
+            return;
+        }
+    } else if (bad) {
+        choose_exactly<T, VPL>(x, top_k, lane, score, expert);
+        return;
+    }
+    const bool got = mine >= kLeast && lane < top_k;
+    expert = got ? static_cast<int>(kExpertBits - (mine & kExpertBits)) : -1;
+    if (kWide) score = got ? to_f32(row[expert]) : -INFINITY;
+    else score = got ? value_of(mine < 0x80000000u ? mine | kExpertBits : mine & ~kExpertBits) : -INFINITY;
+}
+
 template <typename T, int VPL, bool SIGMOID>
 __global__ void __launch_bounds__(kRouterWarps * 32) router_kernel(RouterArgs a, float* __restrict__ weights, int32_t* __restrict__ ids) {
     const int lane = threadIdx.x & 31;
-    const int64_t token = static_cast<int64_t>(blockIdx.x) * kRouterWarps + (threadIdx.x >> 5);
-    if (token >= a.tokens) return;
-    float w = 0.0f;
-    int expert = -1;
-    if (a.mask == nullptr || a.mask[token] != 0) {
-        float x[VPL];
-        load_row<T, VPL>(static_cast<const T*>(a.logits) + token * a.stride, a.experts, a.chunks, lane, x);
-        bool bad = false;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kRouterWarps;
+    for (int64_t token = static_cast<int64_t>(blockIdx.x) * kRouterWarps + (threadIdx.x >> 5); token < a.tokens; token += step) {
+        float w = 0.0f;
+        int expert = -1;
+        if (a.mask == nullptr || a.mask[token] != 0) {
+            float x[VPL];
+            const T* row = static_cast<const T*>(a.logits) + token * a.stride;
+            load_row<T, VPL>(row, a.experts, a.chunks, lane, x);
+            bool bad;
+            float score;
+            choose<T, VPL>(x, row, a.top_k, lane, score, expert, bad);
+            const float u = expert >= 0 ? log_score<SIGMOID>(score) : -INFINITY;
+            if (a.normalize || !SIGMOID) {
+                const float top = __shfl_sync(kAllLanes, u, 0);   // the largest; u rises with the score
+                const float m = top == -INFINITY ? 0.0f : top;
+                const float e = expf(u - m);
+                float s = 0.0f;
+                if (a.normalize) {
+                    s = e;
+                } else {
 #pragma unroll
-        for (int v = 0; v < VPL; ++v) bad |= isnan(x[v]);
-        bad = __any_sync(kAllLanes, bad);
-        float score;
-        choose<T, VPL>(x, a.top_k, lane, score, expert);
-        const float u = expert >= 0 ? log_score<SIGMOID>(score) : -INFINITY;
-        if (a.normalize || !SIGMOID) {
-            const float top = __shfl_sync(kAllLanes, u, 0);   // the largest; u rises with the score
-            const float m = top == -INFINITY ? 0.0f : top;
-            const float e = expf(u - m);
-            float s = 0.0f;
-            if (a.normalize) {
-                s = e;
+                    for (int v = 0; v < VPL; ++v) s += exp_below(x[v] - m);
+                }
+                s = warp_sum(s);
+                w = expert >= 0 ? e / s : 0.0f;
             } else {
-#pragma unroll
-                for (int v = 0; v < VPL; ++v) s += expf(x[v] - m);
+                w = expf(u);
             }
-            s = warp_sum(s);
-            w = expert >= 0 ? e / s : 0.0f;
-        } else {
-            w = expf(u);
+            if (bad) w = NAN;
         }
-        if (bad) w = NAN;
-    }
-    if (lane < a.top_k) {
-        weights[token * a.top_k + lane] = w;
-        ids[token * a.top_k + lane] = expert;
+        if (lane < a.top_k) {
+            weights[token * a.top_k + lane] = w;
+            ids[token * a.top_k + lane] = expert;
+        }
     }
 }
 
@@ -221,23 +321,30 @@ __global__ void __launch_bounds__(kRouterWarps * 32) router_grad_kernel(RouterAr
     const float s = warp_sum(expert >= 0 ? g * w : 0.0f);
     float mine = a.normalize || !SIGMOID ? w * (g - s) : w * g;
     if (SIGMOID && expert >= 0) mine *= sigmoid_of_minus(to_f32(row[expert]));
+    T* out = dlogits + token * a.experts;
+    // the row is put together in shared memory, so that it leaves in full lines
+    __shared__ __align__(16) T put[kRouterWarps][VPL * 32];
+    T* mem = put[threadIdx.x >> 5];
     float x[VPL];
     if (!SIGMOID && !a.normalize && any) {
         load_row<T, VPL>(row, a.experts, a.chunks, lane, x);
-        shares(x);
+        const float inv = exponentials(x);
 #pragma unroll
-        for (int v = 0; v < VPL; ++v) x[v] *= -s;
+        for (int v = 0; v < VPL; ++v) x[v] *= inv * -s;
     } else {
 #pragma unroll
         for (int v = 0; v < VPL; ++v) x[v] = 0.0f;
     }
-    T* out = dlogits + token * a.experts;
-    store_row<T, VPL>(out, a.experts, out_chunks, lane, x);
-    __syncwarp();   // the chosen experts' values after what they replace
-    if (expert >= 0) out[expert] = from_f32<T>(mine);
+    store_row<T, VPL>(mem, VPL * 32, true, lane, x);
+    __syncwarp();
+    if (expert >= 0) mem[expert] = from_f32<T>(mine);
+    __syncwarp();
+    copy_row<T, VPL>(out, mem, a.experts, out_chunks, lane);
 }
 
 // ------------------------------------------------------------------ balance loss
+// A warp's tokens one after another, the next one's ids and scores under way.  A token that names no expert is not
+// read (its scores may be anything).
 struct BalanceArgs {
     const void* logits;
     int64_t tokens, stride;
@@ -245,15 +352,52 @@ struct BalanceArgs {
     bool chunks;
     const int32_t* ids;
 };
-__device__ __forceinline__ bool named(const BalanceArgs& a, int64_t token, int lane, int& expert) {
-    expert = lane < a.top_k ? a.ids[token * a.top_k + lane] : -1;
-    if (expert >= a.experts) expert = -1;
-    return __any_sync(kAllLanes, expert >= 0);
-}
+template <typename T, int VPL>
+struct TokenWalk {
+    const BalanceArgs& a;
+    const int lane;
+    const int64_t step;
+    int64_t token;
+    int expert;      // the lane's, of the token; -1: none
+    bool live;
+    RawRow<T, VPL> raw;
+    __device__ __forceinline__ TokenWalk(const BalanceArgs& args, int l)
+        : a(args), lane(l), step(static_cast<int64_t>(gridDim.x) * kRouterWarps),
+          token(static_cast<int64_t>(blockIdx.x) * kRouterWarps + (threadIdx.x >> 5) - step) {
+        next_id = fetch_id();
+        advance();
+    }
+    __device__ __forceinline__ bool done() const { return token >= a.tokens; }
+    __device__ __forceinline__ void advance() {
+        token += step;
+        expert = next_id;
+        live = __any_sync(kAllLanes, expert >= 0);
+        if (live) raw.load(static_cast<const T*>(a.logits) + token * a.stride, a.experts, a.chunks, lane);
+        next_id = fetch_id();
+    }
 
-// Sums of a block over its tokens: probabilities and pairs of every expert, tokens that count.
+  private:
+    int next_id;
+    __device__ __forceinline__ int fetch_id() const {
+        const int64_t t = token + step;
+        const int e = t < a.tokens && lane < a.top_k ? a.ids[t * a.top_k + lane] : -1;
+        return e < a.experts ? e : -1;
+    }
+};
+
+// What the blocks add up.  Probabilities are added as whole numbers of 2^-shift: whole numbers give the same sum in
+// every order, and with shift = 62 - log2(tokens) a sum is off by less than 2^-50 of its largest.
+struct BalanceSums {
+    unsigned long long* p;   // [experts]
+    int32_t* pairs;          // [experts], then the tokens that count, the blocks that are done, whether a share was NaN
+    int shift;
+};
+
+// Every block adds its tokens' probabilities and pairs; the last one done makes the loss, the counts and
+// coef[e] = E f_e / tokens of the sums.
 template <typename T, int VPL, bool SIGMOID>
-__global__ void __launch_bounds__(kRouterWarps * 32) balance_sums_kernel(BalanceArgs a, float* __restrict__ part_p, int32_t* __restrict__ part_n) {
+__global__ void __launch_bounds__(kRouterWarps * 32) balance_kernel(BalanceArgs a, BalanceSums sums, float* __restrict__ loss, int32_t* __restrict__ counts,
+                                                                   float* __restrict__ coef) {
     using L = RowLayout<T, VPL>;
     extern __shared__ float smem[];
     int32_t* pairs = reinterpret_cast<int32_t*>(smem);                       // [experts], then the tokens that count
@@ -264,74 +408,82 @@ __global__ void __launch_bounds__(kRouterWarps * 32) balance_sums_kernel(Balance
     float acc[VPL];
 #pragma unroll
     for (int v = 0; v < VPL; ++v) acc[v] = 0.0f;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * kRouterWarps;
-    for (int64_t token = static_cast<int64_t>(blockIdx.x) * kRouterWarps + warp; token < a.tokens; token += step) {
-        int expert;
-        if (!named(a, token, lane, expert)) continue;
-        if (expert >= 0) atomicAdd(&pairs[expert], 1);
-        if (lane == 0) atomicAdd(&pairs[a.experts], 1);
+    int tokens = 0;
+    TokenWalk<T, VPL> walk(a, lane);
+    while (!walk.done()) {
+        const bool live = walk.live;
+        const int expert = walk.expert;
         float x[VPL];
-        load_row<T, VPL>(static_cast<const T*>(a.logits) + token * a.stride, a.experts, a.chunks, lane, x);
+        walk.raw.widen(a.experts, lane, x);
+        walk.advance();
+        if (!live) continue;
+        if (expert >= 0) atomicAdd(&pairs[expert], 1);
+        ++tokens;
         if (SIGMOID) {
 #pragma unroll
             for (int v = 0; v < VPL; ++v) x[v] = log_sigmoid(x[v]);
         }
-        shares(x);
+        const float inv = exponentials(x);
 #pragma unroll
-        for (int v = 0; v < VPL; ++v) acc[v] += x[v];
+        for (int v = 0; v < VPL; ++v) acc[v] = fmaf(x[v], inv, acc[v]);
     }
+    if (lane == 0 && tokens != 0) atomicAdd(&pairs[a.experts], tokens);
 #pragma unroll
     for (int v = 0; v < VPL; ++v)
         if (L::expert(v, lane) < a.experts) warp_p[warp * a.experts + L::expert(v, lane)] = acc[v];
     __syncthreads();
+    const float unit = ldexpf(1.0f, sums.shift);
     for (int e = threadIdx.x; e < a.experts; e += blockDim.x) {
         float s = 0.0f;
-        for (int w = 0; w < kRouterWarps; ++w) s += warp_p[w * a.experts + e];
-        part_p[static_cast<int64_t>(blockIdx.x) * a.experts + e] = s;
-    }
-    for (int e = threadIdx.x; e <= a.experts; e += blockDim.x) part_n[static_cast<int64_t>(blockIdx.x) * (a.experts + 1) + e] = pairs[e];
-}
-
-// The blocks' sums in their order (the same bits every time) -> counts, loss, coef[e] = E f_e / tokens.
-__global__ void __launch_bounds__(1024) balance_loss_kernel(const float* __restrict__ part_p, const int32_t* __restrict__ part_n, int blocks, int experts,
-                                                            float* __restrict__ loss, int32_t* __restrict__ counts, float* __restrict__ coef) {
-    __shared__ float warp_s[32];
-    __shared__ long long warp_n[32];
-    __shared__ long long tokens_s;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = threadIdx.x;
-    float p = 0.0f;
-    int32_t n = 0;
-    if (e < experts) {
-        for (int b = 0; b < blocks; ++b) {
-            p += part_p[static_cast<int64_t>(b) * experts + e];
-            n += part_n[static_cast<int64_t>(b) * (experts + 1) + e];
-        }
-        counts[e] = n;
-    }
-    long long total = n, tokens = 0;
-    if (warp == 0) {
-        for (int b = lane; b < blocks; b += 32) tokens += part_n[static_cast<int64_t>(b) * (experts + 1) + experts];
 #pragma unroll
-        for (int d = 16; d > 0; d >>= 1) tokens += __shfl_xor_sync(kAllLanes, tokens, d);
-        if (lane == 0) tokens_s = tokens;
+        for (int w = 0; w < kRouterWarps; ++w) s += warp_p[w * a.experts + e];
+        if (isnan(s)) atomicOr(&sums.pairs[a.experts + 2], 1);
+        else if (s != 0.0f) atomicAdd(&sums.p[e], __float2ull_rn(s * unit));
+        if (pairs[e] != 0) atomicAdd(&sums.pairs[e], pairs[e]);
+    }
+    __threadfence();
+    __syncthreads();
+    __shared__ bool last;
+    if (threadIdx.x == 0) {
+        if (pairs[a.experts] != 0) atomicAdd(&sums.pairs[a.experts], pairs[a.experts]);
+        __threadfence();
+        last = atomicAdd(&sums.pairs[a.experts + 1], 1) == static_cast<int32_t>(gridDim.x) - 1;
+    }
+    __syncthreads();
+    if (!last) return;
+
+    __threadfence();
+    __shared__ long long warp_n[kRouterWarps];
+    __shared__ double warp_s[kRouterWarps];
+    long long all_pairs = 0;
+    for (int e = threadIdx.x; e < a.experts; e += blockDim.x) {
+        const int32_t n = __ldcg(&sums.pairs[e]);
+        counts[e] = n;
+        all_pairs += n;
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) all_pairs += __shfl_xor_sync(kAllLanes, all_pairs, d);
+    if (lane == 0) warp_n[warp] = all_pairs;
+    __syncthreads();
+    all_pairs = 0;
+#pragma unroll
+    for (int w = 0; w < kRouterWarps; ++w) all_pairs += warp_n[w];
+    const int32_t live = __ldcg(&sums.pairs[a.experts]);
+    const float per_token = live > 0 ? static_cast<float>(a.experts) / static_cast<float>(live) : 0.0f;
+    double total = 0.0;
+    for (int e = threadIdx.x; e < a.experts; e += blockDim.x) {
+        const float f = all_pairs > 0 ? static_cast<float>(__ldcg(&sums.pairs[e])) / static_cast<float>(all_pairs) : 0.0f;
+        coef[e] = f * per_token;
+        total += f * static_cast<double>(__ldcg(&sums.p[e]));
     }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(kAllLanes, total, d);
-    if (lane == 0) warp_n[warp] = total;
-    __syncthreads();
-    total = 0;
-    for (int w = 0; w < 32; ++w) total += warp_n[w];
-    tokens = tokens_s;
-    const float f = total > 0 ? static_cast<float>(n) / static_cast<float>(total) : 0.0f;
-    const float per_token = tokens > 0 ? static_cast<float>(experts) / static_cast<float>(tokens) : 0.0f;
-    if (e < experts) coef[e] = f * per_token;
-    const float s = warp_sum(e < experts ? f * p : 0.0f);
-    if (lane == 0) warp_s[warp] = s;
+    if (lane == 0) warp_s[warp] = total;
     __syncthreads();
     if (threadIdx.x == 0) {
-        float all = 0.0f;
-        for (int w = 0; w < 32; ++w) all += warp_s[w];
-        *loss = all * per_token;
+        total = 0.0;
+        for (int w = 0; w < kRouterWarps; ++w) total += warp_s[w];
+        *loss = __ldcg(&sums.pairs[a.experts + 2]) != 0 ? NAN : static_cast<float>(ldexp(total, -sums.shift)) * per_token;
     }
 }
 
@@ -340,35 +492,39 @@ __global__ void __launch_bounds__(kRouterWarps * 32) balance_grad_kernel(Balance
                                                                         T* __restrict__ dlogits, bool out_chunks) {
     using L = RowLayout<T, VPL>;
     const int lane = threadIdx.x & 31;
-    const int64_t token = static_cast<int64_t>(blockIdx.x) * kRouterWarps + (threadIdx.x >> 5);
-    if (token >= a.tokens) return;
-    int expert;
-    float p[VPL];
-    if (named(a, token, lane, expert)) {
-        float x[VPL], c[VPL];
-        load_row<T, VPL>(static_cast<const T*>(a.logits) + token * a.stride, a.experts, a.chunks, lane, x);
-        const float g = *dloss;
-        float inner = 0.0f;
+    const float g = *dloss;
+    float c[VPL];
 #pragma unroll
-        for (int v = 0; v < VPL; ++v) p[v] = log_score<SIGMOID>(x[v]);
-        shares(p);
-#pragma unroll
-        for (int v = 0; v < VPL; ++v) {
-            const int e = L::expert(v, lane);
-            c[v] = e < a.experts ? coef[e] * g : 0.0f;
-            inner += c[v] * p[v];
-        }
-        inner = warp_sum(inner);
-#pragma unroll
-        for (int v = 0; v < VPL; ++v) {
-            p[v] *= c[v] - inner;
-            if (SIGMOID) p[v] *= sigmoid_of_minus(x[v]);
-        }
-    } else {
-#pragma unroll
-        for (int v = 0; v < VPL; ++v) p[v] = 0.0f;
+    for (int v = 0; v < VPL; ++v) {
+        const int e = L::expert(v, lane);
+        c[v] = e < a.experts ? coef[e] * g : 0.0f;
     }
-    store_row<T, VPL>(dlogits + token * a.experts, a.experts, out_chunks, lane, p);
+    TokenWalk<T, VPL> walk(a, lane);
+    while (!walk.done()) {
+        const bool live = walk.live;
+        const int64_t token = walk.token;
+        float x[VPL], p[VPL];
+        walk.raw.widen(a.experts, lane, x);
+        walk.advance();
+        if (live) {
+#pragma unroll
+            for (int v = 0; v < VPL; ++v) p[v] = log_score<SIGMOID>(x[v]);
+            const float inv = exponentials(p);
+            float inner = 0.0f;
+#pragma unroll
+            for (int v = 0; v < VPL; ++v) inner = fmaf(c[v], p[v], inner);
+            inner = warp_sum(inner) * inv;
+#pragma unroll
+            for (int v = 0; v < VPL; ++v) {
+                p[v] *= (c[v] - inner) * inv;
+                if (SIGMOID) p[v] *= sigmoid_of_minus(x[v]);
+            }
+        } else {
+#pragma unroll
+            for (int v = 0; v < VPL; ++v) p[v] = 0.0f;
+        }
+        store_row<T, VPL>(dlogits + token * a.experts, a.experts, out_chunks, lane, p);
+    }
 }
 
 // ------------------------------------------------------------------ launches
@@ -403,11 +559,17 @@ static int check_scores(const void* logits, int dtype, int64_t tokens, int64_t e
 }
 static int launched(const char* what) { return cudaGetLastError() == cudaSuccess ? TGO_OK : route_fail(TGO_E_CUDA, what); }
 static unsigned token_blocks(int64_t tokens) { return static_cast<unsigned>((tokens + kRouterWarps - 1) / kRouterWarps); }
+// for kernels whose warps take one token after another: as many blocks as run at once
+static unsigned resident_blocks(int64_t tokens) {
+    const unsigned b = token_blocks(tokens);
+    return b < 148 * 8 ? b : 148 * 8;
+}
 
-constexpr int64_t kBalanceBlocks = 148 * 2;
-static int64_t balance_blocks(int64_t tokens) {
-    const int64_t b = token_blocks(tokens);
-    return b < kBalanceBlocks ? b : kBalanceBlocks;
+// log2(tokens), rounded up
+static int bits_of(int64_t tokens) {
+    int b = 0;
+    while ((1LL << b) < tokens) ++b;
+    return b;
 }
 
 }  // namespace tgo
@@ -427,8 +589,8 @@ int tgo_moe_router(const void* logits, int dtype, int64_t tokens, int64_t expert
         constexpr int VPL = decltype(vpl)::value;
         const RouterArgs a = {logits, tokens, row_stride, static_cast<int>(experts), static_cast<int>(top_k), normalize != 0,
                               RowLayout<T, VPL>::whole_chunks(logits, experts, row_stride), token_mask};
-        if (scoring == TGO_SCORING_SIGMOID) router_kernel<T, VPL, true><<<token_blocks(tokens), kRouterWarps * 32, 0, st>>>(a, weights, expert_ids);
-        else router_kernel<T, VPL, false><<<token_blocks(tokens), kRouterWarps * 32, 0, st>>>(a, weights, expert_ids);
+        if (scoring == TGO_SCORING_SIGMOID) router_kernel<T, VPL, true><<<resident_blocks(tokens), kRouterWarps * 32, 0, st>>>(a, weights, expert_ids);
+        else router_kernel<T, VPL, false><<<resident_blocks(tokens), kRouterWarps * 32, 0, st>>>(a, weights, expert_ids);
         return launched("router_kernel launch failed");
     });
 }
@@ -456,7 +618,7 @@ int tgo_moe_router_grad(const void* logits, int dtype, int64_t tokens, int64_t e
 
 int64_t tgo_moe_balance_workspace_bytes(int64_t tokens, int64_t experts) {
     if (tokens <= 0 || experts <= 0 || experts > kRouterMaxExperts) return -1;
-    return balance_blocks(tokens) * (2 * experts + 1) * 4;
+    return experts * 12 + 12;
 }
 
 int tgo_moe_balance_loss(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t row_stride, const int32_t* expert_ids,
@@ -468,19 +630,20 @@ int tgo_moe_balance_loss(const void* logits, int dtype, int64_t tokens, int64_t 
     if (rc != TGO_OK) return rc;
     if (workspace_bytes < tgo_moe_balance_workspace_bytes(tokens, experts)) return route_fail(TGO_E_WORKSPACE, "balance workspace too small");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const unsigned blocks = static_cast<unsigned>(balance_blocks(tokens));
-    float* part_p = static_cast<float*>(workspace);
-    int32_t* part_n = reinterpret_cast<int32_t*>(part_p + static_cast<int64_t>(blocks) * experts);
+    if (reinterpret_cast<uintptr_t>(workspace) % 8 != 0) return route_fail(TGO_E_ARG, "the workspace must be 8-byte aligned");
+    const BalanceSums sums = {static_cast<unsigned long long*>(workspace), reinterpret_cast<int32_t*>(static_cast<unsigned long long*>(workspace) + experts),
+                              62 - bits_of(tokens)};
+    if (cudaMemsetAsync(workspace, 0, static_cast<size_t>(experts) * 12 + 12, st) != cudaSuccess) return route_fail(TGO_E_CUDA, "cudaMemsetAsync failed");
+    const unsigned tasks = token_blocks(tokens), blocks = tasks < 148 * 4 ? tasks : 148 * 4;
     const size_t smem = ((kRouterWarps + 1) * experts + 1) * 4;
     return with_layout(dtype, experts, [&](auto t, auto vpl) {
         using T = decltype(t);
         constexpr int VPL = decltype(vpl)::value;
         const BalanceArgs a = {logits, tokens, row_stride, static_cast<int>(experts), static_cast<int>(top_k),
                                RowLayout<T, VPL>::whole_chunks(logits, experts, row_stride), expert_ids};
-        if (scoring == TGO_SCORING_SIGMOID) balance_sums_kernel<T, VPL, true><<<blocks, kRouterWarps * 32, smem, st>>>(a, part_p, part_n);
-        else balance_sums_kernel<T, VPL, false><<<blocks, kRouterWarps * 32, smem, st>>>(a, part_p, part_n);
-        balance_loss_kernel<<<1, 1024, 0, st>>>(part_p, part_n, static_cast<int>(blocks), static_cast<int>(experts), loss, counts, coef);
-        return launched("balance kernel launch failed");
+        if (scoring == TGO_SCORING_SIGMOID) balance_kernel<T, VPL, true><<<blocks, kRouterWarps * 32, smem, st>>>(a, sums, loss, counts, coef);
+        else balance_kernel<T, VPL, false><<<blocks, kRouterWarps * 32, smem, st>>>(a, sums, loss, counts, coef);
+        return launched("balance_kernel launch failed");
     });
 }
 
@@ -498,9 +661,9 @@ int tgo_moe_balance_grad(const void* logits, int dtype, int64_t tokens, int64_t 
         const bool out_chunks = RowLayout<T, VPL>::whole_chunks(d_logits, experts, experts);
         T* out = static_cast<T*>(d_logits);
         if (scoring == TGO_SCORING_SIGMOID)
-            balance_grad_kernel<T, VPL, true><<<token_blocks(tokens), kRouterWarps * 32, 0, st>>>(a, coef, d_loss, out, out_chunks);
+            balance_grad_kernel<T, VPL, true><<<resident_blocks(tokens), kRouterWarps * 32, 0, st>>>(a, coef, d_loss, out, out_chunks);
         else
-            balance_grad_kernel<T, VPL, false><<<token_blocks(tokens), kRouterWarps * 32, 0, st>>>(a, coef, d_loss, out, out_chunks);
+            balance_grad_kernel<T, VPL, false><<<resident_blocks(tokens), kRouterWarps * 32, 0, st>>>(a, coef, d_loss, out, out_chunks);
         return launched("balance_grad_kernel launch failed");
     });
 }
