@@ -32,7 +32,7 @@ def test_the_c_boundary_refuses_before_any_device_work():
         (lambda: balance(ws=8), "workspace"), (lambda: balance(k=0), "top_k"), (lambda: balance(tokens=0), "zero-row"),
         (lambda: dispatch(x=None), "null"), (lambda: dispatch(x=p + 2), "16-byte"), (lambda: dispatch(width=12), "multiple of 8"),
         (lambda: dispatch(experts=4097), "4096"), (lambda: dispatch(k=1025), "1024"), (lambda: dispatch(tokens=1 << 30), "2^31"),
-        (lambda: dispatch(ws=4), "workspace"), (lambda: dispatch(tokens=0), "zero-row"),
+        (lambda: dispatch(tokens=5000, ws=4), "workspace"), (lambda: dispatch(tokens=0), "zero-row"),
         (lambda: lib.tgo_moe_combine(p, -1, p, None, p, 2, 2, 8, None), "negative"), (lambda: lib.tgo_moe_combine(p, 4, p, None, p + 8, 2, 2, 8, None), "16-byte"),
         (lambda: lib.tgo_moe_combine(None, 4, p, None, p, 2, 2, 8, None), "null"),
         (lambda: grad(dy=None), "null"), (lambda: grad(rows=None), "null"), (lambda: grad(d_rows=None, d_w=None), "no gradient"),

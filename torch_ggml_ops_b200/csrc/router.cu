@@ -44,10 +44,14 @@ template <typename T, int VPL>
 struct RawRow {
     using L = RowLayout<T, VPL>;
     Pack<T, L::CH> p[VPL / L::CH];
+    // -inf beyond the last expert
     __device__ __forceinline__ void load(const T* __restrict__ row, int experts, bool chunks, int lane) {
+        const T none = from_f32<T>(-INFINITY);
 #pragma unroll
         for (int c = 0; c < VPL / L::CH; ++c) {
             const int e = L::expert(c * L::CH, lane);
+#pragma unroll
+            for (int j = 0; j < L::CH; ++j) p[c].v[j] = none;
             if (chunks) {
                 if (e < experts) p[c] = *reinterpret_cast<const Pack<T, L::CH>*>(row + e);
             } else {
@@ -57,17 +61,16 @@ struct RawRow {
             }
         }
     }
-    // x[v] = the scores, -inf beyond the last expert
-    __device__ __forceinline__ void widen(int experts, int lane, float (&x)[VPL]) const {
+    __device__ __forceinline__ void widen(float (&x)[VPL]) const {
 #pragma unroll
-        for (int v = 0; v < VPL; ++v) x[v] = L::expert(v, lane) < experts ? to_f32(p[v / L::CH].v[v % L::CH]) : -INFINITY;
+        for (int v = 0; v < VPL; ++v) x[v] = to_f32(p[v / L::CH].v[v % L::CH]);
     }
 };
 template <typename T, int VPL>
 __device__ __forceinline__ void load_row(const T* __restrict__ row, int experts, bool chunks, int lane, float (&x)[VPL]) {
     RawRow<T, VPL> raw;
     raw.load(row, experts, chunks, lane);
-    raw.widen(experts, lane, x);
+    raw.widen(x);
 }
 template <typename T, int VPL>
 __device__ __forceinline__ void store_row(T* __restrict__ row, int experts, bool chunks, int lane, const float (&x)[VPL]) {
@@ -144,7 +147,9 @@ __device__ __forceinline__ float exponentials(float (&u)[VPL]) {
         s += u[v];
     }
     s = warp_sum(s);
-    return s == 0.0f ? 0.0f : 1.0f / s;
+    float inv;   // of a sum of 1 at least
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+    return s == 0.0f ? 0.0f : inv;
 }
 
 struct RouterArgs {
@@ -220,6 +225,7 @@ __device__ __forceinline__ void choose(const float (&x)[VPL], const T* __restric
     for (int v = 1; v < VPL; ++v) first = max(first, key[v]);
     uint32_t mine = 0, low = 0, left = first;
     const int slots = kWide && top_k < 32 ? top_k + 1 : top_k;   // fp32: whether the next one is as large has to be seen
+#pragma unroll 8
     for (int s = 0; s < slots; ++s) {
         low = __reduce_max_sync(kAllLanes, left);
         if (lane == s) mine = low;
@@ -263,12 +269,13 @@ template <typename T, int VPL, bool SIGMOID>
 __global__ void __launch_bounds__(kRouterWarps * 32) router_kernel(RouterArgs a, float* __restrict__ weights, int32_t* __restrict__ ids) {
     const int lane = threadIdx.x & 31;
     const int64_t step = static_cast<int64_t>(gridDim.x) * kRouterWarps;
-    for (int64_t token = static_cast<int64_t>(blockIdx.x) * kRouterWarps + (threadIdx.x >> 5); token < a.tokens; token += step) {
+    int64_t token = static_cast<int64_t>(blockIdx.x) * kRouterWarps + (threadIdx.x >> 5);
+    const T* row = static_cast<const T*>(a.logits) + token * a.stride;
+    for (; token < a.tokens; token += step, row += step * a.stride) {
         float w = 0.0f;
         int expert = -1;
         if (a.mask == nullptr || a.mask[token] != 0) {
             float x[VPL];
-            const T* row = static_cast<const T*>(a.logits) + token * a.stride;
             load_row<T, VPL>(row, a.experts, a.chunks, lane, x);
             bool bad;
             float score;
@@ -414,7 +421,7 @@ __global__ void __launch_bounds__(kRouterWarps * 32) balance_kernel(BalanceArgs 
         const bool live = walk.live;
         const int expert = walk.expert;
         float x[VPL];
-        walk.raw.widen(a.experts, lane, x);
+        walk.raw.widen(x);
         walk.advance();
         if (!live) continue;
         if (expert >= 0) atomicAdd(&pairs[expert], 1);
@@ -504,7 +511,7 @@ __global__ void __launch_bounds__(kRouterWarps * 32) balance_grad_kernel(Balance
         const bool live = walk.live;
         const int64_t token = walk.token;
         float x[VPL], p[VPL];
-        walk.raw.widen(a.experts, lane, x);
+        walk.raw.widen(x);
         walk.advance();
         if (live) {
 #pragma unroll

@@ -255,10 +255,10 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> dispatch_cuda(const Tensor& x, const 
     Tensor indices = at::empty({experts}, i64), offsets = at::empty({experts}, i32);
     const int64_t bytes = tgo_moe_dispatch_workspace_bytes(pairs, experts);
     TORCH_CHECK(bytes >= 0, "unsupported sizes");
-    Tensor ws = at::empty({bytes}, i32.dtype(at::kByte));
+    const Tensor ws = bytes > 0 ? at::empty({bytes}, i32.dtype(at::kByte)) : Tensor();
     check_rc(tgo_moe_dispatch(x.const_data_ptr(), ids.const_data_ptr<int32_t>(), tokens, k, experts, h, rows.mutable_data_ptr(),
                               at_row.mutable_data_ptr<int32_t>(), indices.mutable_data_ptr<int64_t>(), offsets.mutable_data_ptr<int32_t>(),
-                              ws.mutable_data_ptr(), bytes, stream_of(x)),
+                              bytes > 0 ? ws.mutable_data_ptr() : nullptr, bytes, stream_of(x)),
              "moe_dispatch");
     return {rows, at_row, indices, offsets};
 }
