@@ -124,6 +124,14 @@ def test_router_shows_nan(cuda, scoring, normalize):
     x[3, 5] = math.inf
     w, ids = tgo.moe_router(x.cuda(), 4, scoring=scoring, normalize=normalize)
     assert torch.isnan(w[1]).all() and torch.isnan(w[2]).all() and bool((ids[2] == -1).all()) and 9 not in ids[1]
+    y = scores(6, 50, torch.float32)
+    y.view(torch.int32)[4, 49] = -1                       # a NaN with its sign set
+    for dtype in DTYPES:
+        z = y.to(dtype)
+        if dtype != torch.float32:
+            z.view(torch.int16)[4, 49] = -1
+        wy, idy = tgo.moe_router(z.cuda(), 4, scoring=scoring, normalize=normalize)
+        assert torch.isnan(wy[4]).all() and 49 not in idy[4] and bool(torch.isfinite(wy[:4]).all())
     assert int(ids[3, 0]) == 5 and (torch.isnan(w[3, 0]) if scoring == "softmax" else bool(torch.isfinite(w[3]).all()))
     for t in (0, 4, 5):
         assert torch.equal(w[t], clean[t]) and torch.equal(ids[t], clean_ids[t])
@@ -157,6 +165,51 @@ def test_router_layouts(cuda):
     e = torch.empty(0, 77, device="cuda", requires_grad=True)
     w6, ids6 = tgo.moe_router(e, 3)
     assert w6.shape == (0, 3) and ids6.shape == (0, 3) and torch.autograd.grad(w6.sum(), e)[0].shape == (0, 77)
+
+
+@pytest.mark.parametrize("scoring,normalize", [("softmax", True), ("softmax", False), ("sigmoid", True), ("sigmoid", False)])
+def test_router_gradient_against_differences(cuda, scoring, normalize):
+    import torch_ggml_ops_b200 as tgo
+
+    x = scores(8, 12, torch.float32, 6)
+    g = torch.randn(8, 3, generator=torch.Generator().manual_seed(1))
+    xd = x.cuda().requires_grad_()
+    w, ids = tgo.moe_router(xd, 3, scoring=scoring, normalize=normalize)
+    (dx,) = torch.autograd.grad(w, xd, g.cuda())
+    h = 2.0 ** -11                                        # no two scores are as near, so the choice stays
+    for t in range(8):
+        for e in range(12):
+            ends = []
+            for step in (h, -h):
+                y = x[t:t + 1].double().clone()
+                y[0, e] += step
+                wy, iy = ref.router(y, 3, scoring, normalize)
+                assert torch.equal(iy[0], ids[t].cpu())
+                ends.append(float((wy[0] * g[t].double()).sum()))
+            # third derivatives of the weights are below 1: h^2 / 6 of the cotangent's size, and fp32
+            assert abs((ends[0] - ends[1]) / (2 * h) - float(dx[t, e])) < 1e-6 * (1 + float(g[t].abs().sum()))
+
+
+def test_combine_gradients_against_differences(cuda):
+    """The sums are linear in the rows and in the weights: the change of <out, dy> is the gradient, up to the sums' roundings."""
+    import torch_ggml_ops_b200 as tgo
+
+    g = torch.Generator().manual_seed(12)
+    at = ref.sort_rows(expert_ids(6, 3, 8, 5, 0.2), 8)[0]
+    rows, w = torch.randn(18, 16, generator=g).bfloat16(), torch.randn(6, 3, generator=g)
+    dy = torch.randn(6, 16, generator=g).bfloat16()
+    rd, wd = rows.cuda().requires_grad_(), w.cuda().requires_grad_()
+    d_rows, d_w = torch.autograd.grad(tgo.moe_combine(rd, at.cuda(), wd), [rd, wd], dy.cuda())
+    value = lambda r, v: float((ref.combine(r, at, v)[0] * dy.double()).sum())   # noqa: E731
+    base = value(rows, w)
+    for t, s in ((0, 0), (2, 1), (5, 2)):
+        moved = w.double().clone()
+        moved[t, s] += 1.0
+        assert abs(value(rows, moved) - base - float(d_w[t, s])) < 1e-4
+    for r, c in ((0, 0), (7, 3), (17, 15)):
+        moved = rows.double().clone()
+        moved[r, c] += 1.0
+        assert abs(value(moved, w) - base - float(d_rows[r, c])) <= 2.0 ** -8 * abs(float(d_rows[r, c])) + 1e-9
 
 
 def test_refusals(cuda):

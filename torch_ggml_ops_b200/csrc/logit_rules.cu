@@ -8,7 +8,14 @@
 // One block per slice of a row's vocabulary: it brings the slice's logits to shared memory, counts the history's
 // tokens that fall into the slice meanwhile, amends the logits of the tokens that history or biases name and
 // writes the slice out under the mask.  One launch, no table of counts in memory; every slice reads all of its row's
-// history (from L2).
+// history, from L2, and that is what bounds long ones.  us on one B200 (248320 tokens; in a graph, one call after another):
+//   16 rows bf16 (15.9 MB)      logits alone 4.7, mask 4.8, 16 biases 5.8, 512 ids 7.4, 4096 10.7, 16384 16.2
+//   200 rows bf16 (199 MB)      16 ids 42 (4.7 TB/s), 512 50, 4096 65, 16384 122
+//   200 rows fp32 (397 MB)      logits alone 63.4 (6.3 TB/s, as a copy), mask 65.1, mask and 1500 ids 89
+// Tried: a pass under the mask and a second kernel for the named tokens, with a hash table or ranks in a bit table, that starts
+// while the first runs (16 rows 14.2 to 26, 200 rows fp32 81: its phases are latency, and short histories got slower);
+// clusters of eight blocks that share one reading of the history (all but the longest slower); the history sorted by
+// slices first (a block per row: 5 us and more, as much of a history is in few slices).
 #include "../../include/tgo_mmq.h"
 
 #include <atomic>
@@ -19,7 +26,6 @@ namespace tgo {
 
 int route_fail(int code, const char* msg);  // tgo_api.cu
 
-constexpr int kRulesThreads = 256;
 constexpr int kRulesPad = 16;   // a row's first elements, in front of its first 16-byte boundary
 
 struct RulesArgs {
@@ -51,17 +57,17 @@ __device__ __forceinline__ uint32_t distance(uint2 id, uint32_t lo, uint32_t spa
 // f(d[kAhead]) for the distances of ids, by the block's whole warps, where a lane has one: several ids are
 // under way per thread, so that the loop waits for L2 once in so many.
 constexpr int kAhead = 8;
-template <typename Id, typename F>
+template <int THREADS, typename Id, typename F>
 __device__ __forceinline__ void each_id(const Id* __restrict__ ids, int64_t n, uint32_t lo, uint32_t span, F f) {
     const int lane = threadIdx.x & 31;
     ids += threadIdx.x;
-    for (int64_t left = n - (threadIdx.x - lane); left > 0; left -= kRulesThreads * kAhead, ids += kRulesThreads * kAhead) {
+    for (int64_t left = n - (threadIdx.x - lane); left > 0; left -= THREADS * kAhead, ids += THREADS * kAhead) {
         Id id[kAhead];
         uint32_t d[kAhead];
         bool any = false;
-        if (left >= kRulesThreads * (kAhead - 1) + 32) {
+        if (left >= THREADS * (kAhead - 1) + 32) {
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) id[u] = ids[u * kRulesThreads];
+            for (int u = 0; u < kAhead; ++u) id[u] = ids[u * THREADS];
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
                 d[u] = distance(id[u], lo, span);
@@ -71,10 +77,10 @@ __device__ __forceinline__ void each_id(const Id* __restrict__ ids, int64_t n, u
             const int mine = static_cast<int>(left) - lane;
 #pragma unroll
             for (int u = 0; u < kAhead; ++u)
-                if (u * kRulesThreads < mine) id[u] = ids[u * kRulesThreads];
+                if (u * THREADS < mine) id[u] = ids[u * THREADS];
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
-                d[u] = u * kRulesThreads < mine ? distance(id[u], lo, span) : kNone;
+                d[u] = u * THREADS < mine ? distance(id[u], lo, span) : kNone;
                 any |= d[u] != kNone;
             }
         }
@@ -90,7 +96,7 @@ __device__ __forceinline__ float penalised(float x, uint32_t count, const Penalt
 }
 
 // What a block works on, from the row's first 16-byte boundary on in vectors
-template <typename T>
+template <typename T, int THREADS>
 struct Slice {
     static constexpr int VEC = 16 / static_cast<int>(sizeof(T));
     static constexpr uint32_t kAll = (1u << VEC) - 1u;
@@ -126,25 +132,25 @@ struct Slice {
     __device__ __forceinline__ void finish(const RulesArgs& a, X x, S same, O one) const {
         auto put = [&](int64_t t) { out[t] = words == nullptr || (words[t >> 5] >> (t & 31) & 1u) != 0 ? one(t) : from_f32<T>(-INFINITY); };
         if (!a.vectors) {
-            for (int64_t t = lo + threadIdx.x; t < hi; t += kRulesThreads) put(t);
+            for (int64_t t = lo + threadIdx.x; t < hi; t += THREADS) put(t);
             return;
         }
         edges(put);
         const int n = vecs();
         constexpr int kDeep = 4;
-        for (int v0 = threadIdx.x; v0 < n; v0 += kRulesThreads * kDeep) {
+        for (int v0 = threadIdx.x; v0 < n; v0 += THREADS * kDeep) {
             Pack<T, VEC> p[kDeep];
             uint32_t bits[kDeep], w[2][kDeep];
             bool skip[kDeep];
 #pragma unroll
             for (int u = 0; u < kDeep; ++u) {
-                const int64_t t = base + static_cast<int64_t>(v0 + u * kRulesThreads) * VEC;
+                const int64_t t = base + static_cast<int64_t>(v0 + u * THREADS) * VEC;
                 w[0][u] = w[1][u] = 0xFFFFFFFFu;
-                if (words != nullptr && v0 + u * kRulesThreads < n) w[0][u] = words[t >> 5], w[1][u] = words[(t + VEC - 1) >> 5];
+                if (words != nullptr && v0 + u * THREADS < n) w[0][u] = words[t >> 5], w[1][u] = words[(t + VEC - 1) >> 5];
             }
 #pragma unroll
             for (int u = 0; u < kDeep; ++u) {
-                const int v = v0 + u * kRulesThreads;
+                const int v = v0 + u * THREADS;
                 bits[u] = __funnelshift_r(w[0][u], w[1][u], static_cast<uint32_t>((base + static_cast<int64_t>(v) * VEC) & 31)) & kAll;
                 skip[u] = v >= n || (bits[u] == kAll && same(v));
                 if (!skip[u] && bits[u] != 0) p[u] = x(v);
@@ -155,31 +161,32 @@ struct Slice {
 #pragma unroll
                 for (int j = 0; j < VEC; ++j)
                     if ((bits[u] >> j & 1u) == 0) p[u].v[j] = from_f32<T>(-INFINITY);
-                *reinterpret_cast<Pack<T, VEC>*>(out + base + static_cast<int64_t>(v0 + u * kRulesThreads) * VEC) = p[u];
+                *reinterpret_cast<Pack<T, VEC>*>(out + base + static_cast<int64_t>(v0 + u * THREADS) * VEC) = p[u];
             }
         }
     }
 };
 
 // the mask alone
+constexpr int kMaskThreads = 256;
 template <typename T>
-__global__ void __launch_bounds__(kRulesThreads, 4) logit_mask_kernel(RulesArgs a) {
-    const Slice<T> s(a);
-    using Vec = Pack<T, Slice<T>::VEC>;
+__global__ void __launch_bounds__(kMaskThreads, 4) logit_mask_kernel(RulesArgs a) {
+    const Slice<T, kMaskThreads> s(a);
+    using Vec = Pack<T, Slice<T, kMaskThreads>::VEC>;
     s.finish(
-        a, [&](int v) { return *reinterpret_cast<const Vec*>(s.in + s.base + static_cast<int64_t>(v) * Slice<T>::VEC); }, [&](int) { return a.in_place; },
+        a, [&](int v) { return *reinterpret_cast<const Vec*>(s.in + s.base + static_cast<int64_t>(v) * Slice<T, kMaskThreads>::VEC); }, [&](int) { return a.in_place; },
         [&](int64_t t) { return s.in[t]; });
 }
 
 // C: type of a count; 16 bits where no history is longer than they count.  Shared memory: the slice's logits, its
 // counts, its biases, each from token base - kRulesPad on; then the tokens that history or biases name, each once, so that the
 // arithmetic runs on 32 of them at a time however thinly they lie.
-template <typename T, typename C>
-__global__ void __launch_bounds__(kRulesThreads, 4) logit_rules_kernel(RulesArgs a) {
+template <typename T, typename C, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) logit_rules_kernel(RulesArgs a) {
     extern __shared__ uint4 smem[];
     __shared__ int n_named;
-    const Slice<T> s(a);
-    constexpr int VEC = Slice<T>::VEC;
+    const Slice<T, THREADS> s(a);
+    constexpr int VEC = Slice<T, THREADS>::VEC;
     const int tokens = a.slice + kRulesPad, lane = threadIdx.x & 31;
     const bool counting = a.history != nullptr, biased = a.bias_ids != nullptr;
     T* x = reinterpret_cast<T*>(smem);
@@ -188,7 +195,7 @@ __global__ void __launch_bounds__(kRulesThreads, 4) logit_rules_kernel(RulesArgs
     uint16_t* named = reinterpret_cast<uint16_t*>(biased ? bias + tokens : bias);
 
     // the logits on their way while the tables are made
-    for (int v = threadIdx.x; v < s.vecs(); v += kRulesThreads)
+    for (int v = threadIdx.x; v < s.vecs(); v += THREADS)
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<unsigned>(__cvta_generic_to_shared(x + kRulesPad + v * VEC))),
                      "l"(s.in + s.base + static_cast<int64_t>(v) * VEC)
                      : "memory");
@@ -208,7 +215,7 @@ __global__ void __launch_bounds__(kRulesThreads, 4) logit_rules_kernel(RulesArgs
     {
         uint4* table = reinterpret_cast<uint4*>(count);
         const int chunks = tokens * static_cast<int>((counting ? sizeof(C) : 0) + (biased ? 4 : 0)) / 16;
-        for (int i = threadIdx.x; i < chunks; i += kRulesThreads) table[i] = make_uint4(0, 0, 0, 0);
+        for (int i = threadIdx.x; i < chunks; i += THREADS) table[i] = make_uint4(0, 0, 0, 0);
         if (threadIdx.x == 0) n_named = 0;
         __syncthreads();
     }
@@ -245,8 +252,8 @@ __global__ void __launch_bounds__(kRulesThreads, 4) logit_rules_kernel(RulesArgs
     };
     if (counting) {
         const int64_t at = s.row * a.history_stride;
-        if (a.history_wide) each_id(static_cast<const uint2*>(a.history) + at, n, static_cast<uint32_t>(s.lo), span, add);
-        else each_id(static_cast<const uint32_t*>(a.history) + at, n, static_cast<uint32_t>(s.lo), span, add);
+        if (a.history_wide) each_id<THREADS>(static_cast<const uint2*>(a.history) + at, n, static_cast<uint32_t>(s.lo), span, add);
+        else each_id<THREADS>(static_cast<const uint32_t*>(a.history) + at, n, static_cast<uint32_t>(s.lo), span, add);
     }
     if (biased) __syncthreads();
     if (biased && threadIdx.x < 32) {
@@ -281,7 +288,7 @@ __global__ void __launch_bounds__(kRulesThreads, 4) logit_rules_kernel(RulesArgs
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
 
-    for (int j = threadIdx.x; j < n_named; j += kRulesThreads) {
+    for (int j = threadIdx.x; j < n_named; j += THREADS) {
         const int i = named[j];
         const float b = biased ? bias[i] : 0.0f;
         const uint32_t c = counting ? count[i] : 0u;
@@ -305,39 +312,44 @@ __global__ void __launch_bounds__(kRulesThreads, 4) logit_rules_kernel(RulesArgs
 }
 
 // ------------------------------------------------------------------ launches
-constexpr int64_t kRulesMemory = 55 * 1024;   // shared memory of a block: four of them on an SM
+constexpr int64_t kThreadMemory = 220;   // bytes of shared memory per thread: an SM's for 1024
 
-template <typename T, typename C>
+template <typename T, typename C, int THREADS>
 static int launch_slices(const RulesArgs& a, size_t smem, cudaStream_t st) {
     static std::atomic<bool> ready[64];   // a kernel may use more than 48 KB only after a call per device has said so
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return route_fail(TGO_E_CUDA, "cudaGetDevice failed");
     if (dev >= 64 || !ready[dev].load(std::memory_order_relaxed)) {
-        if (cudaFuncSetAttribute(logit_rules_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kRulesMemory)) != cudaSuccess)
+        if (cudaFuncSetAttribute(logit_rules_kernel<T, C, THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kThreadMemory * THREADS)) != cudaSuccess)
             return route_fail(TGO_E_CUDA, "cudaFuncSetAttribute failed");
         if (dev < 64) ready[dev].store(true, std::memory_order_relaxed);
     }
-    logit_rules_kernel<T, C><<<static_cast<unsigned>(a.rows * a.slices), kRulesThreads, smem, st>>>(a);
+    logit_rules_kernel<T, C, THREADS><<<static_cast<unsigned>(a.rows * a.slices), THREADS, smem, st>>>(a);
     return cudaGetLastError() == cudaSuccess ? TGO_OK : route_fail(TGO_E_CUDA, "logit_rules_kernel launch failed");
 }
 
 template <typename T>
 static int launch_rules(RulesArgs& a, int64_t id_bytes, cudaStream_t st) {
     const bool tables = a.history != nullptr || a.bias_ids != nullptr, narrow = a.history_len <= UINT16_MAX;
+    // Every slice reads all of a history, so that of a long one larger slices read less; small ones overlap their phases better
+    // (us with 256 / 512 threads, bf16, 248320 tokens: 16 rows of 1024 ids 7.6 / 10.1, of 4096 10.7 / 10.7, of 16384 20.3 / 16.1;
+    // 200 rows of 1024 ids 51.5 / 57.7, of 4096 68.7 / 64.9, of 16384 162 / 122; 1024 threads are slower but for the longest).
+    const int threads = a.history_len < 4096 ? 256 : 512;
     const int64_t token_bytes = static_cast<int64_t>(sizeof(T)) + (a.history != nullptr ? (narrow ? 2 : 4) : 0) + (a.bias_ids != nullptr ? 4 : 0);
     // the list of named tokens is as long as history and biases together, or as the slice
-    const int64_t all_names = a.history_len + a.n_bias;
+    const int64_t all_names = a.history_len + a.n_bias, memory = kThreadMemory * threads;
     int64_t most = 16384;
     if (tables) {
-        const int64_t long_list = kRulesMemory / (token_bytes + 2), short_list = all_names < kRulesMemory ? (kRulesMemory - 2 * all_names) / token_bytes : 0;
+        const int64_t long_list = memory / (token_bytes + 2), short_list = all_names < memory ? (memory - 2 * all_names) / token_bytes : 0;
         most = ((long_list > short_list ? long_list : short_list) - kRulesPad - 1) / 128 * 128;
+        if (most > 65536 - 256) most = 65536 - 256;   // the list holds 16 bits of a token
     }
-    // some four blocks per SM, no slice shorter than 1024 tokens, none longer than its shared memory takes
-    int64_t slices = (148 * 4 + a.rows - 1) / a.rows;
-    if (slices > (a.vocab + 1023) / 1024) slices = (a.vocab + 1023) / 1024;
+    // some 1024 threads per SM, no slice shorter than 4 tokens per thread, none longer than its shared memory takes
+    int64_t slices = (148 * (1024 / threads) + a.rows - 1) / a.rows;
+    if (slices > (a.vocab + 4 * threads - 1) / (4 * threads)) slices = (a.vocab + 4 * threads - 1) / (4 * threads);
     if (a.history != nullptr) {
-        // Of a long history that every slice reads: so few slices that it is no more than twice what they read and write else, down to a
-        // block per SM (us with / without, bf16: 4 rows of 65535 ids 27.9 / 39.3, 16 rows 38.4 / 53.0; 16 rows of 4096 ids 14.3 / 14.4).
+        // Of a long history so few slices that they read no more than twice as much of it as they read and write else, down to a
+        // block per SM (us with / without, bf16: 4 rows of 8192 ids 7.2 / 9.1, of 65535 25.8 / 37.0; 16 rows of 16384 16.2 / 17.9).
         const int64_t fair = 4 * a.vocab * static_cast<int64_t>(sizeof(T)) / (a.history_len * id_bytes), fewest = (148 + a.rows - 1) / a.rows;
         if (slices > fair) slices = fair > fewest ? fair : fewest < slices ? fewest : slices;
     }
@@ -347,12 +359,13 @@ static int launch_rules(RulesArgs& a, int64_t id_bytes, cudaStream_t st) {
     a.slice = static_cast<int>(((a.vocab + slices - 1) / slices + 127) / 128 * 128);
     if (!tables) {
         if (a.in_place && a.allowed == nullptr) return TGO_OK;
-        logit_mask_kernel<T><<<static_cast<unsigned>(a.rows * slices), kRulesThreads, 0, st>>>(a);
+        logit_mask_kernel<T><<<static_cast<unsigned>(a.rows * slices), kMaskThreads, 0, st>>>(a);
         return cudaGetLastError() == cudaSuccess ? TGO_OK : route_fail(TGO_E_CUDA, "logit_mask_kernel launch failed");
     }
     const int64_t names = all_names < a.slice + kRulesPad ? all_names : a.slice + kRulesPad;
     const size_t smem = static_cast<size_t>(token_bytes) * (a.slice + kRulesPad) + static_cast<size_t>(names) * 2;
-    return narrow ? launch_slices<T, uint16_t>(a, smem, st) : launch_slices<T, uint32_t>(a, smem, st);
+    if (threads == 256) return launch_slices<T, uint16_t, 256>(a, smem, st);
+    return narrow ? launch_slices<T, uint16_t, 512>(a, smem, st) : launch_slices<T, uint32_t, 512>(a, smem, st);
 }
 
 }  // namespace tgo

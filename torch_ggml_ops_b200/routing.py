@@ -103,7 +103,7 @@ def moe_dispatch(input: torch.Tensor, expert_ids: torch.Tensor, num_experts: int
     row_of_pair, expert_indices, expert_offsets)``.  ``rows`` [pairs, width] with the last two are what
     ``grouped_mmq``, ``grouped_mmq_pair`` and ``moe_mlp`` take (every expert a group, empty ones too; up to 4096
     experts).  ``row_of_pair`` (int32, like ``expert_ids`` [..., top_k]): each pair's row, for ``moe_combine``; -1 for
-    pairs whose id names no expert.  Rows behind the last expert's are zeros, and none of the grouped products.
+    pairs whose id names no expert.  Rows behind the last expert's are zeros; the grouped products leave theirs as they are.
 
     ``rows`` is differentiable with respect to ``input`` (the pairs' gradients are added in fp32)."""
     return _ops.moe_dispatch.default(input, expert_ids, num_experts)
