@@ -14,8 +14,18 @@
 //
 // One warp per token, the row in its registers: lane l holds chunks of consecutive experts, so that a
 // row is read once, in full lines.
+//
+// Measured on one B200, GPU time in a graph (us), 256 experts, top 8, bf16 (floor: scores in or out at 6.4 TB/s, 5.2 us for 65536 tokens):
+//   router      16 tokens 2.3, 65536 29.4;  gradient 65536 12.3 (normalised)
+//   balance     65536 24;  gradient 65536 23 (floor 10.4)
+//   fp32: router 8200 tokens 6.8, gradient of the plain probabilities 3.7;  1291 tokens of 1000 experts, top 4, 4.6
+// What bounds the router: instructions (345 per token, 69 % of the issue slots): keys 40, eight choices 50, the scores put in
+// after them 50, softmax and result 60.  Choosing by (score, expert) with two reductions and a search of the registers
+// took 61 us, two cached scores per lane with a refill 36.  The balance loss has some 8 us that do not shrink with the
+// tokens (clearing the sums, adding them across blocks, the last block's work) and 160 instructions per token.
 #include "../../include/tgo_mmq.h"
 
+#include <atomic>
 #include <type_traits>
 
 #include "scores.cuh"
@@ -193,26 +203,35 @@ __device__ __noinline__ void choose_exactly(const float (&x)[VPL], int top_k, in
     }
 }
 
+template <int VPL>
+__device__ __forceinline__ uint32_t largest(const uint32_t (&k)[VPL]) {
+    uint32_t m = k[0];
+#pragma unroll
+    for (int v = 1; v + 1 < VPL; v += 2) m = __vimax3_u32(m, k[v], k[v + 1]);
+    return VPL % 2 == 0 ? max(m, k[VPL - 1]) : m;
+}
+
 // the largest of a lane's keys that is below `last`, one of them; 0 if there is none.  Keys below last wrap around
 // to the largest differences.
 template <int VPL>
 __device__ __forceinline__ uint32_t next_below(const uint32_t (&key)[VPL], uint32_t last) {
-    uint32_t m = key[0] - last;
+    uint32_t d[VPL];
 #pragma unroll
-    for (int v = 1; v < VPL; ++v) m = max(m, key[v] - last);
-    return m + last < last ? m + last : 0u;
+    for (int v = 0; v < VPL; ++v) d[v] = key[v] - last;
+    const uint32_t m = largest(d) + last;
+    return m < last ? m : 0u;
 }
 
 // The same with one reduction per choice and no search for the expert: a key holds the upper 22 bits of a score's
 // order and, below, the expert (the lower expert the larger number), so that no two are equal.  That is all of a
 // 16-bit score.  Of two fp32 scores that agree in the 22 bits the exact comparison decides: a row where such are
 // among the best (1 in 70 of 256 normal scores) goes through choose_exactly.
-// First the best top_k of the lanes' best, in order; lane s holds the s-th.  Scores of the same lanes that belong
+// First the best top_k of the lanes' best, in order, by way of `slot` in shared memory; lane s holds the s-th.  Scores of the same lanes that belong
 // among them (one or two in a row as a rule) are then put in one by one.
 // bad: the row holds a NaN (its order, like any NaN's after the addition of 0, is above all).
 constexpr uint32_t kExpertBits = 1023;
 template <typename T, int VPL>
-__device__ __forceinline__ void choose(const float (&x)[VPL], const T* __restrict__ row, int top_k, int lane, float& score, int& expert, bool& bad) {
+__device__ __forceinline__ void choose(const float (&x)[VPL], const T* __restrict__ row, int top_k, int lane, uint32_t* slot, float& score, int& expert, bool& bad) {
     using L = RowLayout<T, VPL>;
     constexpr bool kWide = sizeof(T) == 4;
     constexpr uint32_t kLeast = 0x00800000u;     // order of the lowest finite fp32 (fp16's and bf16's are no lower): -inf is below
@@ -220,17 +239,22 @@ __device__ __forceinline__ void choose(const float (&x)[VPL], const T* __restric
     uint32_t key[VPL];
 #pragma unroll
     for (int v = 0; v < VPL; ++v) key[v] = (order_of(x[v]) & ~kExpertBits) | (kExpertBits - L::expert(v, lane));
-    uint32_t first = key[0];
-#pragma unroll
-    for (int v = 1; v < VPL; ++v) first = max(first, key[v]);
-    uint32_t mine = 0, low = 0, left = first;
+    const uint32_t first = largest(key);
+    uint32_t low = 0, left = first;
     const int slots = kWide && top_k < 32 ? top_k + 1 : top_k;   // fp32: whether the next one is as large has to be seen
+    slot[lane] = 0;
+    __syncwarp();
 #pragma unroll 8
     for (int s = 0; s < slots; ++s) {
         low = __reduce_max_sync(kAllLanes, left);
-        if (lane == s) mine = low;
-        if (left == low) left = 0;
+        if (left == low) {
+            slot[s] = low;
+            left = 0;
+        }
     }
+    __syncwarp();
+    uint32_t mine = slot[lane];
+    __syncwarp();
     bad = __shfl_sync(kAllLanes, mine, 0) > (kInfinite | kExpertBits);
     if (VPL > 1) {
         // `low` is the least that is in; a lane whose best is out has nothing that is better
@@ -267,6 +291,7 @@ __device__ __forceinline__ void choose(const float (&x)[VPL], const T* __restric
 
 template <typename T, int VPL, bool SIGMOID>
 __global__ void __launch_bounds__(kRouterWarps * 32) router_kernel(RouterArgs a, float* __restrict__ weights, int32_t* __restrict__ ids) {
+    __shared__ uint32_t slots[kRouterWarps][32];
     const int lane = threadIdx.x & 31;
     const int64_t step = static_cast<int64_t>(gridDim.x) * kRouterWarps;
     int64_t token = static_cast<int64_t>(blockIdx.x) * kRouterWarps + (threadIdx.x >> 5);
@@ -279,7 +304,7 @@ __global__ void __launch_bounds__(kRouterWarps * 32) router_kernel(RouterArgs a,
             load_row<T, VPL>(row, a.experts, a.chunks, lane, x);
             bool bad;
             float score;
-            choose<T, VPL>(x, row, a.top_k, lane, score, expert, bad);
+            choose<T, VPL>(x, row, a.top_k, lane, slots[threadIdx.x >> 5], score, expert, bad);
             const float u = expert >= 0 ? log_score<SIGMOID>(score) : -INFINITY;
             if (a.normalize || !SIGMOID) {
                 const float top = __shfl_sync(kAllLanes, u, 0);   // the largest; u rises with the score
@@ -567,9 +592,16 @@ static int check_scores(const void* logits, int dtype, int64_t tokens, int64_t e
 static int launched(const char* what) { return cudaGetLastError() == cudaSuccess ? TGO_OK : route_fail(TGO_E_CUDA, what); }
 static unsigned token_blocks(int64_t tokens) { return static_cast<unsigned>((tokens + kRouterWarps - 1) / kRouterWarps); }
 // for kernels whose warps take one token after another: as many blocks as run at once
-static unsigned resident_blocks(int64_t tokens) {
+template <auto KERNEL>
+static unsigned resident_blocks(int64_t tokens, size_t smem = 0) {
+    static std::atomic<int> per_sm{0};
+    int n = per_sm.load(std::memory_order_relaxed);
+    if (n == 0) {
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, KERNEL, kRouterWarps * 32, smem) != cudaSuccess || n < 1) n = 1;
+        per_sm.store(n, std::memory_order_relaxed);
+    }
     const unsigned b = token_blocks(tokens);
-    return b < 148 * 8 ? b : 148 * 8;
+    return b < 148u * n ? b : 148u * n;
 }
 
 // log2(tokens), rounded up
@@ -596,8 +628,8 @@ int tgo_moe_router(const void* logits, int dtype, int64_t tokens, int64_t expert
         constexpr int VPL = decltype(vpl)::value;
         const RouterArgs a = {logits, tokens, row_stride, static_cast<int>(experts), static_cast<int>(top_k), normalize != 0,
                               RowLayout<T, VPL>::whole_chunks(logits, experts, row_stride), token_mask};
-        if (scoring == TGO_SCORING_SIGMOID) router_kernel<T, VPL, true><<<resident_blocks(tokens), kRouterWarps * 32, 0, st>>>(a, weights, expert_ids);
-        else router_kernel<T, VPL, false><<<resident_blocks(tokens), kRouterWarps * 32, 0, st>>>(a, weights, expert_ids);
+        if (scoring == TGO_SCORING_SIGMOID) router_kernel<T, VPL, true><<<resident_blocks<router_kernel<T, VPL, true>>(tokens), kRouterWarps * 32, 0, st>>>(a, weights, expert_ids);
+        else router_kernel<T, VPL, false><<<resident_blocks<router_kernel<T, VPL, false>>(tokens), kRouterWarps * 32, 0, st>>>(a, weights, expert_ids);
         return launched("router_kernel launch failed");
     });
 }
@@ -641,15 +673,14 @@ int tgo_moe_balance_loss(const void* logits, int dtype, int64_t tokens, int64_t 
     const BalanceSums sums = {static_cast<unsigned long long*>(workspace), reinterpret_cast<int32_t*>(static_cast<unsigned long long*>(workspace) + experts),
                               62 - bits_of(tokens)};
     if (cudaMemsetAsync(workspace, 0, static_cast<size_t>(experts) * 12 + 12, st) != cudaSuccess) return route_fail(TGO_E_CUDA, "cudaMemsetAsync failed");
-    const unsigned tasks = token_blocks(tokens), blocks = tasks < 148 * 4 ? tasks : 148 * 4;
     const size_t smem = ((kRouterWarps + 1) * experts + 1) * 4;
     return with_layout(dtype, experts, [&](auto t, auto vpl) {
         using T = decltype(t);
         constexpr int VPL = decltype(vpl)::value;
         const BalanceArgs a = {logits, tokens, row_stride, static_cast<int>(experts), static_cast<int>(top_k),
                                RowLayout<T, VPL>::whole_chunks(logits, experts, row_stride), expert_ids};
-        if (scoring == TGO_SCORING_SIGMOID) balance_kernel<T, VPL, true><<<blocks, kRouterWarps * 32, smem, st>>>(a, sums, loss, counts, coef);
-        else balance_kernel<T, VPL, false><<<blocks, kRouterWarps * 32, smem, st>>>(a, sums, loss, counts, coef);
+        if (scoring == TGO_SCORING_SIGMOID) balance_kernel<T, VPL, true><<<resident_blocks<balance_kernel<T, VPL, true>>(tokens, smem), kRouterWarps * 32, smem, st>>>(a, sums, loss, counts, coef);
+        else balance_kernel<T, VPL, false><<<resident_blocks<balance_kernel<T, VPL, false>>(tokens, smem), kRouterWarps * 32, smem, st>>>(a, sums, loss, counts, coef);
         return launched("balance_kernel launch failed");
     });
 }
@@ -668,9 +699,9 @@ int tgo_moe_balance_grad(const void* logits, int dtype, int64_t tokens, int64_t 
         const bool out_chunks = RowLayout<T, VPL>::whole_chunks(d_logits, experts, experts);
         T* out = static_cast<T*>(d_logits);
         if (scoring == TGO_SCORING_SIGMOID)
-            balance_grad_kernel<T, VPL, true><<<resident_blocks(tokens), kRouterWarps * 32, 0, st>>>(a, coef, d_loss, out, out_chunks);
+            balance_grad_kernel<T, VPL, true><<<resident_blocks<balance_grad_kernel<T, VPL, true>>(tokens), kRouterWarps * 32, 0, st>>>(a, coef, d_loss, out, out_chunks);
         else
-            balance_grad_kernel<T, VPL, false><<<resident_blocks(tokens), kRouterWarps * 32, 0, st>>>(a, coef, d_loss, out, out_chunks);
+            balance_grad_kernel<T, VPL, false><<<resident_blocks<balance_grad_kernel<T, VPL, false>>(tokens), kRouterWarps * 32, 0, st>>>(a, coef, d_loss, out, out_chunks);
         return launched("balance_grad_kernel launch failed");
     });
 }
