@@ -80,8 +80,17 @@ def test_router_of_nearly_equal_scores(cuda):
     for i in range(x.shape[0]):
         b = base[i % 7].view(torch.int32) + torch.randint(0, 4 if i < 21 else 4000, (200,), generator=g, dtype=torch.int32)
         x[i] = b.view(torch.float32)
-    for k in (1, 8, 20):
+    for k in (1, 8, 20, 32):
         check_router(x, k, "softmax", True, grad=False)
+    # equal numbers among the best, and one behind them that is larger by the last bit only
+    y = torch.zeros(64, 70)
+    for i in range(64):
+        y[i, : i + 3] = 2.0
+        y[i, i + 5] = torch.nextafter(torch.tensor(2.0), torch.tensor(3.0))
+        y[i, 69] = torch.nextafter(torch.tensor(2.0), torch.tensor(1.0))
+    for k in (1, 4, 7, 31, 32):
+        check_router(y, k, "sigmoid", True, grad=False)
+        check_router(scores(30, 70, torch.float32, k).bfloat16().float(), k, "softmax", False, grad=False)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -131,7 +131,7 @@ __device__ __forceinline__ float warp_max(const float (&x)[VPL]) {
     float m = x[0];
 #pragma unroll
     for (int v = 1; v < VPL; ++v) m = fmaxf(m, x[v]);
-    asm("redux.sync.max.f32 %0, %0, 0xffffffff;" : "+f"(m));
+    asm volatile("redux.sync.max.f32 %0, %0, 0xffffffff;" : "+f"(m));
     return m;
 }
 
@@ -224,10 +224,10 @@ __device__ __forceinline__ uint32_t next_below(const uint32_t (&key)[VPL], uint3
 
 // The same with one reduction per choice and no search for the expert: a key holds the upper 22 bits of a score's
 // order and, below, the expert (the lower expert the larger number), so that no two are equal.  That is all of a
-// 16-bit score.  Of two fp32 scores that agree in the 22 bits the exact comparison decides: a row where such are
-// among the best (1 in 70 of 256 normal scores) goes through choose_exactly.
-// First the best top_k of the lanes' best, in order, by way of `slot` in shared memory; lane s holds the s-th.  Scores of the same lanes that belong
-// among them (one or two in a row as a rule) are then put in one by one.
+// 16-bit score.  Of two different fp32 scores that agree in the 22 bits the exact comparison decides: a row where such
+// are among the best (1 in 70 of 256 normal scores) goes through choose_exactly.
+// First the best top_k of the lanes' best, in order, by way of `slot` in shared memory; lane s holds the s-th.  Scores of
+// the same lanes that belong among them (one or two in a row as a rule) are then put in one by one.
 // bad: the row holds a NaN (its order, like any NaN's after the addition of 0, is above all).
 constexpr uint32_t kExpertBits = 1023;
 template <typename T, int VPL>
@@ -267,19 +267,23 @@ __device__ __forceinline__ void choose(const float (&x)[VPL], const T* __restric
             if (next == put) next = next_below(key, put);
         }
     }
+    bool search = bad;
     if (kWide) {
-        // the last of 32 has no slot behind it: whether another one is as large is looked up
         const uint32_t above = __shfl_up_sync(kAllLanes, mine, 1);
-        bool close = lane > 0 && lane < slots && mine >= kLeast && ((mine ^ above) & ~kExpertBits) == 0;
-        if (top_k == 32) {
+        const bool alike = lane > 0 && lane < slots && mine >= kLeast && ((mine ^ above) & ~kExpertBits) == 0;
+        if (__any_sync(kAllLanes, alike) || top_k == 32) {   // the last of 32 has no slot behind it
+            // Equal numbers are in order already (fp32 scores that were rounded to bf16 often are equal): those in the slots are compared
+            // with the one above, the others that are like the last slot's with it.
+            const float x0 = lane < slots && mine >= kLeast ? to_f32(row[kExpertBits - (mine & kExpertBits)]) : 0.0f;
+            const float x1 = __shfl_up_sync(kAllLanes, x0, 1);
+            bool differ = alike && x0 != x1;
+            const uint32_t last = order_of(__shfl_sync(kAllLanes, x0, slots - 1));
 #pragma unroll
-            for (int v = 0; v < VPL; ++v) close |= ((key[v] ^ low) & ~kExpertBits) == 0 && key[v] < low;
+            for (int v = 0; v < VPL; ++v) differ |= low >= kLeast && ((key[v] ^ low) & ~kExpertBits) == 0 && order_of(x[v]) != last;
+            search |= __any_sync(kAllLanes, differ);
         }
-        if (__any_sync(kAllLanes, close) || bad) {
-            choose_exactly<T, VPL>(x, top_k, lane, score, expert);
-            return;
-        }
-    } else if (bad) {
+    }
+    if (search) {
         choose_exactly<T, VPL>(x, top_k, lane, score, expert);
         return;
     }
