@@ -6,8 +6,8 @@
 //
 // All of it is bound by memory: a token's row is read once and its top_k rows are written (or read) once.  One B200, rows of
 // 2048, top 8, GPU time in a graph (bytes that have to move over it):
-//   dispatch 16384 tokens 116 us (5.2 TB/s; the rows alone 98, 6.2 TB/s), its gradient 97 (6.2)
-//   combine 600 tokens 4.5 us, 8192 51.8 (5.8 TB/s), its gradients 102.3 (5.6; the main kernel 97)
+//   dispatch 16384 tokens 116 us (5.2 TB/s; the rows alone 98, 6.2 TB/s), its gradient 93.8 (6.4)
+//   combine 600 tokens 4.4 us, 8192 48.6 (6.2 TB/s), its gradients 97.6 (5.9)
 // A copy runs at 6.4.
 #include "../../include/tgo_mmq.h"
 
@@ -211,19 +211,31 @@ __global__ void __launch_bounds__(kMoveThreads) dispatch_rows_kernel(const uint4
 __global__ void __launch_bounds__(kMoveThreads) moe_combine_kernel(const uint4* __restrict__ rows, long long n_rows, const int32_t* __restrict__ row_of_pair,
                                                                    const float* __restrict__ weights, uint4* __restrict__ out, long long tokens,
                                                                    int top_k, int vec_per_row) {
+    constexpr int kDeep = 4;   // rows under way per thread (8192 tokens, one row / four: 51.8 / 48.6 us)
     const long long step = static_cast<long long>(kMoveThreads) * gridDim.x;
     for (long long v = blockIdx.x * static_cast<long long>(kMoveThreads) + threadIdx.x; v < tokens * vec_per_row; v += step) {
         const long long t = v / vec_per_row;
         const int c = static_cast<int>(v - t * vec_per_row);
         float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        for (int s = 0; s < top_k; ++s) {
-            const int row = row_of_pair[t * top_k + s];
-            if (row < 0 || row >= n_rows) continue;
-            const float w = weights != nullptr ? weights[t * top_k + s] : 1.0f;
-            float f[8];
-            widen(rows[static_cast<long long>(row) * vec_per_row + c], f);
+        for (int s0 = 0; s0 < top_k; s0 += kDeep) {
+            uint4 q[kDeep];
+            float w[kDeep];
+            bool in[kDeep];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) acc[j] = fmaf(w, f[j], acc[j]);
+            for (int u = 0; u < kDeep; ++u) {
+                const int row = s0 + u < top_k ? row_of_pair[t * top_k + s0 + u] : -1;
+                in[u] = row >= 0 && row < n_rows;
+                if (in[u]) q[u] = rows[static_cast<long long>(row) * vec_per_row + c];
+                w[u] = in[u] && weights != nullptr ? weights[t * top_k + s0 + u] : 1.0f;
+            }
+#pragma unroll
+            for (int u = 0; u < kDeep; ++u) {
+                if (!in[u]) continue;
+                float f[8];
+                widen(q[u], f);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) acc[j] = fmaf(w[u], f[j], acc[j]);
+            }
         }
         out[v] = narrow(acc);
     }
@@ -257,19 +269,33 @@ __global__ void __launch_bounds__(kMoveThreads) combine_grad_kernel(const uint4*
         const uint4* r = rows + static_cast<long long>(row) * vec_per_row;
         const bool alone = d_rows == nullptr || count[row] == 1;
         const float w = weights != nullptr ? weights[pair] : 1.0f;
-        for (int c = lane; c < vec_per_row; c += 32) {
-            float f[8];
-            widen(g[c], f);
-            if (d_weights != nullptr) {
-                float h[8];
-                widen(r[c], h);
+        constexpr int kDeep = 4;   // chunks under way per lane (gradients of 8192 tokens, 1 / 2 / 4 / 8 chunks: 102 / 109 / 98 / 130 us)
+        for (int c0 = lane; c0 < vec_per_row; c0 += 32 * kDeep) {
+            uint4 dyv[kDeep], rowv[kDeep];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) dot = fmaf(f[j], h[j], dot);
+            for (int u = 0; u < kDeep; ++u) {
+                const int c = c0 + 32 * u;
+                if (c >= vec_per_row) continue;
+                dyv[u] = g[c];
+                if (d_weights != nullptr) rowv[u] = r[c];
             }
-            if (d_rows != nullptr && alone) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) f[j] *= w;
-                d_rows[static_cast<long long>(row) * vec_per_row + c] = narrow(f);
+            for (int u = 0; u < kDeep; ++u) {
+                const int c = c0 + 32 * u;
+                if (c >= vec_per_row) continue;
+                float f[8];
+                widen(dyv[u], f);
+                if (d_weights != nullptr) {
+                    float h[8];
+                    widen(rowv[u], h);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) dot = fmaf(f[j], h[j], dot);
+                }
+                if (d_rows != nullptr && alone) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) f[j] *= w;
+                    d_rows[static_cast<long long>(row) * vec_per_row + c] = narrow(f);
+                }
             }
         }
         if (!alone) {
