@@ -59,7 +59,7 @@ std::tuple<Tensor, Tensor> router_cuda(const Tensor& logits, int64_t top_k, int6
     }
     const c10::cuda::CUDAGuard guard(logits.device());
     const auto sizes = with_last(logits.sizes(), top_k);
-    Tensor w = at::empty(sizes, logits.options().dtype(at::kFloat)), ids = at::empty(sizes, logits.options().dtype(at::kInt));
+    Tensor w = new_cuda(sizes, at::kFloat, logits), ids = new_cuda(sizes, at::kInt, logits);
     if (r.rows > 0)
         check_rc(tgo_moe_router(logits.const_data_ptr(), code, r.rows, r.width, r.stride, top_k, static_cast<int>(scoring), normalize,
                                 mask.has_value() ? reinterpret_cast<const uint8_t*>(mask->const_data_ptr<bool>()) : nullptr,
@@ -78,7 +78,7 @@ Tensor router_grad_cuda(const Tensor& grad, const Tensor& logits, const Tensor& 
     check_router(r, w.size(-1), scoring);
     const c10::cuda::CUDAGuard guard(logits.device());
     const Tensor d = grad.contiguous();
-    Tensor dx = at::empty(logits.sizes(), logits.options());
+    Tensor dx = new_cuda(logits.sizes(), logits.scalar_type(), logits);
     if (r.rows > 0)
         check_rc(tgo_moe_router_grad(logits.const_data_ptr(), code, r.rows, r.width, r.stride, ids.const_data_ptr<int32_t>(),
                                      w.const_data_ptr<float>(), d.const_data_ptr<float>(), w.size(-1), static_cast<int>(scoring), normalize,
@@ -154,10 +154,10 @@ std::tuple<Tensor, Tensor, Tensor> balance_cuda(const Tensor& logits, const Tens
     const c10::cuda::CUDAGuard guard(logits.device());
     const auto f32 = logits.options().dtype(at::kFloat);
     if (r.rows == 0) return {at::zeros({}, f32), at::zeros({r.width}, f32.dtype(at::kInt)), at::zeros({r.width}, f32)};
-    Tensor loss = at::empty({}, f32), counts = at::empty({r.width}, f32.dtype(at::kInt)), coef = at::empty({r.width}, f32);
+    Tensor loss = new_cuda({}, at::kFloat, logits), counts = new_cuda({r.width}, at::kInt, logits), coef = new_cuda({r.width}, at::kFloat, logits);
     const int64_t bytes = tgo_moe_balance_workspace_bytes(r.rows, r.width);
     TORCH_CHECK(bytes >= 0, "unsupported sizes");
-    Tensor ws = at::empty({bytes}, f32.dtype(at::kByte));
+    Tensor ws = new_cuda({bytes}, at::kByte, logits);
     check_rc(tgo_moe_balance_loss(logits.const_data_ptr(), code, r.rows, r.width, r.stride, ids.const_data_ptr<int32_t>(), ids.size(-1),
                                   static_cast<int>(scoring), loss.mutable_data_ptr<float>(), counts.mutable_data_ptr<int32_t>(),
                                   coef.mutable_data_ptr<float>(), ws.mutable_data_ptr(), bytes, stream_of(logits)),
@@ -174,7 +174,7 @@ Tensor balance_grad_cuda(const Tensor& grad, const Tensor& logits, const Tensor&
     check_plain(grad, logits, at::kFloat, "grad");
     TORCH_CHECK(grad.numel() == 1, "grad must be one number");
     const c10::cuda::CUDAGuard guard(logits.device());
-    Tensor dx = at::empty(logits.sizes(), logits.options());
+    Tensor dx = new_cuda(logits.sizes(), logits.scalar_type(), logits);
     if (r.rows > 0)
         check_rc(tgo_moe_balance_grad(logits.const_data_ptr(), code, r.rows, r.width, r.stride, ids.const_data_ptr<int32_t>(), ids.size(-1),
                                       static_cast<int>(scoring), coef.const_data_ptr<float>(), grad.const_data_ptr<float>(),
@@ -250,12 +250,12 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> dispatch_cuda(const Tensor& x, const 
     TORCH_CHECK(experts >= 1 && experts <= 4096, "num_experts must be in 1..4096; got ", experts);
     const c10::cuda::CUDAGuard guard(x.device());
     const auto i32 = ids.options(), i64 = i32.dtype(at::kLong);
-    Tensor rows = at::empty({pairs, h}, x.options()), at_row = at::empty(ids.sizes(), i32);
+    Tensor rows = new_cuda({pairs, h}, at::kBFloat16, x), at_row = new_cuda(ids.sizes(), at::kInt, x);
     if (pairs == 0) return {rows, at_row, at::arange(experts, i64), at::zeros({experts}, i32)};
-    Tensor indices = at::empty({experts}, i64), offsets = at::empty({experts}, i32);
+    Tensor indices = new_cuda({experts}, at::kLong, x), offsets = new_cuda({experts}, at::kInt, x);
     const int64_t bytes = tgo_moe_dispatch_workspace_bytes(pairs, experts);
     TORCH_CHECK(bytes >= 0, "unsupported sizes");
-    const Tensor ws = bytes > 0 ? at::empty({bytes}, i32.dtype(at::kByte)) : Tensor();
+    const Tensor ws = bytes > 0 ? new_cuda({bytes}, at::kByte, x) : Tensor();
     check_rc(tgo_moe_dispatch(x.const_data_ptr(), ids.const_data_ptr<int32_t>(), tokens, k, experts, h, rows.mutable_data_ptr(),
                               at_row.mutable_data_ptr<int32_t>(), indices.mutable_data_ptr<int64_t>(), offsets.mutable_data_ptr<int32_t>(),
                               bytes > 0 ? ws.mutable_data_ptr() : nullptr, bytes, stream_of(x)),
@@ -280,7 +280,7 @@ Tensor combine_cuda(const Tensor& rows, const Tensor& at_row, const std::optiona
     const c10::cuda::CUDAGuard guard(rows.device());
     const auto sizes = with_last(at_row.sizes(), h);
     if (rows.size(0) == 0) return at::zeros(sizes, rows.options());
-    Tensor out = at::empty(sizes, rows.options());
+    Tensor out = new_cuda(sizes, at::kBFloat16, rows);
     if (tokens > 0)
         check_rc(tgo_moe_combine(rows.const_data_ptr(), rows.size(0), at_row.const_data_ptr<int32_t>(),
                                  w.has_value() ? w->const_data_ptr<float>() : nullptr, out.mutable_data_ptr(), tokens, k, h, stream_of(rows)),
@@ -298,13 +298,12 @@ std::tuple<Tensor, Tensor> combine_grad_cuda(const Tensor& grad, const Tensor& r
                 "grad must be a torch.bfloat16 tensor like the result");
     Tensor d = grad.contiguous();
     if (reinterpret_cast<uintptr_t>(d.const_data_ptr()) % 16 != 0) d = d.clone();
-    const auto f32 = rows.options().dtype(at::kFloat);
-    Tensor d_rows = at::empty({need_rows ? rows.size(0) : 0, h}, rows.options());
-    Tensor d_w = need_weights ? at::empty(at_row.sizes(), f32) : at::empty({0}, f32);
+    Tensor d_rows = new_cuda({need_rows ? rows.size(0) : 0, h}, at::kBFloat16, rows);
+    Tensor d_w = need_weights ? new_cuda(at_row.sizes(), at::kFloat, rows) : new_cuda({0}, at::kFloat, rows);
     if (rows.size(0) == 0 || tokens == 0) return {d_rows.zero_(), d_w.zero_()};
     if (!need_rows && !need_weights) return {d_rows, d_w};
     const int64_t bytes = need_rows ? rows.size(0) * 4 : 0;
-    Tensor ws = at::empty({bytes}, f32.dtype(at::kByte));
+    const Tensor ws = bytes > 0 ? new_cuda({bytes}, at::kByte, rows) : Tensor();
     check_rc(tgo_moe_combine_grad(d.const_data_ptr(), rows.const_data_ptr(), rows.size(0), at_row.const_data_ptr<int32_t>(),
                                   w.has_value() ? w->const_data_ptr<float>() : nullptr, need_rows ? d_rows.mutable_data_ptr() : nullptr,
                                   need_weights ? d_w.mutable_data_ptr<float>() : nullptr, tokens, k, h, bytes > 0 ? ws.mutable_data_ptr() : nullptr,
@@ -469,8 +468,10 @@ void rules_into(const Tensor& logits, const MaybeTensor& history, const MaybeTen
 Tensor rules_cuda(const Tensor& logits, const MaybeTensor& history, const MaybeTensor& lengths, const MaybeTensor& repetition, double repetition_all,
                   const MaybeTensor& presence, double presence_all, const MaybeTensor& frequency, double frequency_all, const MaybeTensor& bias_ids,
                   const MaybeTensor& bias_values, const MaybeTensor& allowed) {
+    type_code(logits);   // refused before anything is allocated
+    TORCH_CHECK(logits.is_cuda(), "logits must be a CUDA tensor");
     const c10::cuda::CUDAGuard guard(logits.device());
-    Tensor out = at::empty(logits.sizes(), logits.options());
+    Tensor out = new_cuda(logits.sizes(), logits.scalar_type(), logits);
     rules_into(logits, history, lengths, repetition, repetition_all, presence, presence_all, frequency, frequency_all, bias_ids, bias_values, allowed, out);
     return out;
 }
