@@ -207,6 +207,15 @@ def test_refusals(cuda):
     base = torch.randn(4, 64, device="cuda")
     with pytest.raises(RuntimeError, match="overlap|memory"):
         tgo.logit_rules(base[:3], out=base[1:])
+    wide = torch.randn(3, 300, device="cuda")
+    for bad in (wide[:, 8:72], wide[:, 63:127], wide.reshape(-1)[:192].reshape(3, 64)):
+        with pytest.raises(RuntimeError, match="no memory"):
+            tgo.logit_rules(wide[:, :64], out=bad)
+    beside = wide[:, 64:128]
+    assert torch.equal(tgo.logit_rules(wide[:, :64], bias_ids=h[0], bias_values=torch.ones(4, device="cuda"), out=beside),
+                       tgo.logit_rules(wide[:, :64], bias_ids=h[0], bias_values=torch.ones(4, device="cuda")))
+    with pytest.raises(RuntimeError, match="overlap|memory"):
+        tgo.logit_rules(base, bias_ids=h[0], bias_values=base[0, :4], out=base)
     with pytest.raises(RuntimeError, match="contiguous"):
         tgo.logit_rules(torch.randn(64, 3, device="cuda").t())
     with pytest.raises(RuntimeError, match="rows, vocab"):
@@ -240,6 +249,11 @@ def test_captured_and_on_other_streams(cuda):
     assert torch.equal(out, call(c)) and not torch.equal(out, want)
     compiled = torch.compile(lambda x, h: tgo.logit_rules(x, history=h, presence_penalty=0.5), fullgraph=True, backend="aot_eager")
     assert torch.equal(compiled(c["logits"], c["history"]), tgo.logit_rules(c["logits"], history=c["history"], presence_penalty=0.5))
+    ops = torch.ops.torch_ggml_ops_b200
+    args = (c["logits"], c["history"], None, None, 1.1, None, 0.0, None, 0.5, None, None, None)
+    tests = ("test_schema", "test_autograd_registration", "test_faketensor")
+    torch.library.opcheck(ops.logit_rules.default, args, test_utils=tests)
+    torch.library.opcheck(ops.logit_rules_out.default, (*args, torch.empty_like(c["logits"])), test_utils=tests)
     inplace = torch.compile(lambda x, h: tgo.logit_rules(x, history=h, presence_penalty=0.5, out=x), fullgraph=True, backend="aot_eager")
     x = c["logits"].clone()
     inplace(x, c["history"])

@@ -418,6 +418,7 @@ int tgo_moe_combine_grad(const void* dy, const void* rows, int64_t n_rows, const
     int32_t* count = static_cast<int32_t*>(workspace);
     int64_t items = pairs;
     if (d_rows != nullptr) {
+        if (reinterpret_cast<uintptr_t>(workspace) % 4 != 0) return route_fail(TGO_E_ARG, "the workspace must be 4-byte aligned");
         if (workspace == nullptr || workspace_bytes < n_rows * 4) return route_fail(TGO_E_WORKSPACE, "combine workspace is smaller than n_rows * 4 bytes");
         if (cudaMemsetAsync(count, 0, static_cast<size_t>(n_rows) * 4, st) != cudaSuccess) return route_fail(TGO_E_CUDA, "cudaMemsetAsync failed");
         count_rows_kernel<<<static_cast<unsigned>((pairs + kMoveThreads - 1) / kMoveThreads), kMoveThreads, 0, st>>>(row_of_pair, pairs, n_rows, count);
