@@ -9,13 +9,15 @@
 // tokens that fall into the slice meanwhile, amends the logits of the tokens that history or biases name and
 // writes the slice out under the mask.  One launch, no table of counts in memory; every slice reads all of its row's
 // history, from L2, and that is what bounds long ones.  us on one B200 (248320 tokens; in a graph, one call after another):
-//   16 rows bf16 (15.9 MB)      logits alone 4.7, mask 4.8, 16 biases 5.8, 512 ids 7.4, 4096 10.7, 16384 16.2
+//   16 rows bf16 (15.9 MB)      logits alone 4.7, mask 4.8, 16 biases 5.8, 512 ids 7.4, 4096 10.7, 16384 16.2;
+//                               ragged histories up to 8192, biases and mask 13.8
 //   200 rows bf16 (199 MB)      16 ids 42 (4.7 TB/s), 512 50, 4096 65, 16384 122
 //   200 rows fp32 (397 MB)      logits alone 63.4 (6.3 TB/s, as a copy), mask 65.1, mask and 1500 ids 89
 // Tried: a pass under the mask and a second kernel for the named tokens, with a hash table or ranks in a bit table, that starts
 // while the first runs (16 rows 14.2 to 26, 200 rows fp32 81: its phases are latency, and short histories got slower);
 // clusters of eight blocks that share one reading of the history (all but the longest slower); the history sorted by
-// slices first (a block per row: 5 us and more, as much of a history is in few slices).
+// slices first (a block per row: 5 us and more, as much of a history is in few slices); larger slices with the tables alone in
+// shared memory, looked up in the pass vector by vector (16 rows of 8192 ids, biases and mask 16.9 for 13.8, 200 rows of 16 ids 62 for 42).
 #include "../../include/tgo_mmq.h"
 
 #include <atomic>
