@@ -287,3 +287,18 @@ def test_a_decode_step(cuda):
             assert int(token[0]) == 103
             history[:, step] = token
             hidden = (hidden.float() * 0.9 + y.float() * 0.01).bfloat16()
+
+
+def test_offsets_beyond_32_bits(cuda):
+    import torch_ggml_ops_b200 as tgo
+
+    rows, vocab = 2 ** 31 // 248320 + 3, 248320
+    x = torch.ones(rows, vocab, dtype=torch.bfloat16, device="cuda")
+    h = torch.tensor([5, vocab - 1], device="cuda").expand(rows, 2)
+    words = torch.full((rows, vocab // 32), -1, dtype=torch.int32, device="cuda")
+    words[-1, 0] = ~4
+    y = tgo.logit_rules(x, history=h, repetition_penalty=2.0, allowed=words)
+    assert float(y[-1, 5]) == float(y[-1, -1]) == float(y[0, 5]) == 0.5 and float(y[-1, 2]) == -math.inf
+    assert int((y[-1] == 1).sum()) == vocab - 3 and int((y[-2] == 1).sum()) == vocab - 2
+    tgo.logit_rules(x, history=h, repetition_penalty=2.0, allowed=words, out=x)
+    assert torch.equal(x[-2:], y[-2:]) and torch.equal(x[:2], y[:2])

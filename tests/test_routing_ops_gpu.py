@@ -319,14 +319,14 @@ def test_balance_loss_without_tokens(cuda):
     ids = torch.zeros(9, 2, dtype=torch.int32, device="cuda")
     ids[2] = -1
     loss, _ = tgo.moe_balance_loss(x, ids)
-    assert math.isfinite(float(loss)) and bool(torch.isfinite(torch.autograd.grad(loss, x)[0]).all())
+    assert math.isfinite(float(loss.detach())) and bool(torch.isfinite(torch.autograd.grad(loss, x)[0]).all())
     # a row with every expert switched off that names one all the same
     y = scores(3, 12, torch.float32).cuda()
     y[1] = -math.inf
     y.requires_grad_()
     loss, _ = tgo.moe_balance_loss(y, ids[:3] * 0)
     (dy,) = torch.autograd.grad(loss, y)
-    assert math.isfinite(float(loss)) and not dy[1].any() and bool(torch.isfinite(dy).all())
+    assert math.isfinite(float(loss.detach())) and not dy[1].any() and bool(torch.isfinite(dy).all())
 
 
 def test_an_even_use_costs_one(cuda):
@@ -672,3 +672,36 @@ def test_compiled_and_checked_by_torch(cuda):
                      (ops.moe_router_grad, (torch.rand(6, 2, device="cuda"), logits.detach(), ids, w.detach(), 0, True)),
                      (ops.moe_combine_grad, (rows[:6].detach(), rows.detach(), at, w.detach(), True, False))):
         torch.library.opcheck(op.default, args, test_utils=tests)
+
+
+def test_offsets_beyond_32_bits(cuda):
+    """More than 2^31 scores, and rows of more than 2^31 elements: what is behind them is found."""
+    import torch_ggml_ops_b200 as tgo
+
+    tokens = 2 ** 31 // 512 + 5
+    x = torch.zeros(tokens, 512, dtype=torch.bfloat16, device="cuda")
+    x[-3:, 100] = 4.0
+    x[-3:, 511] = 3.0
+    x.requires_grad_()
+    w, ids = tgo.moe_router(x, 2, normalize=False)
+    assert ids[-3:].tolist() == [[100, 511]] * 3 and ids[:3].tolist() == [[0, 1]] * 3
+    (dx,) = torch.autograd.grad(w[-1, 0], x)
+    assert not dx[:-1].any() and float(dx[-1, 100]) > 0 > float(dx[-1, 511])
+    loss, counts = tgo.moe_balance_loss(x, ids)
+    assert counts[[0, 1, 100, 511]].tolist() == [tokens - 3, tokens - 3, 3, 3]
+    (dx,) = torch.autograd.grad(loss, x)
+    assert float(dx[-1, 0]) > 0 and torch.equal(dx[0], dx[-4])
+    del x, dx
+    tokens = 2 ** 31 // (2 * 2048) + 3
+    t = torch.zeros(tokens, 2048, dtype=torch.bfloat16, device="cuda")
+    t[-1] = 1.0
+    t.requires_grad_()
+    ids = torch.zeros(tokens, 2, dtype=torch.int32, device="cuda")
+    ids[:, 1] = 1
+    rows, at, _, ends = tgo.moe_dispatch(t, ids, 2)
+    assert at[-1].tolist() == [tokens - 1, 2 * tokens - 1] and ends.tolist() == [tokens, 2 * tokens]
+    assert bool((rows[-1] == 1).all()) and bool((rows[tokens - 1] == 1).all()) and not rows[tokens:-1].any()
+    y = tgo.moe_combine(rows, at, torch.full((tokens, 2), 0.75, device="cuda"))
+    assert bool((y[-1] == 1.5).all()) and not y[:-1].any()
+    (dt,) = torch.autograd.grad(y[-1].sum(), t)
+    assert bool((dt[-1] == 1.5).all()) and not dt[:-1].any()
