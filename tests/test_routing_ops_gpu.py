@@ -648,6 +648,45 @@ def test_second_derivatives_are_refused(cuda):
         dr.float().sum().backward()
 
 
+def test_what_autograd_keeps(cuda):
+    """Two passes over one graph, a second one after it was freed, inputs that were written over, forward mode, hooks on what is kept."""
+    import torch_ggml_ops_b200 as tgo
+
+    x = torch.randn(5, 8, device="cuda", requires_grad=True)
+    ids = torch.arange(10, dtype=torch.int32, device="cuda").reshape(5, 2) % 8
+    t = torch.randn(5, 16, device="cuda").bfloat16().requires_grad_()
+    rows, at, _, _ = tgo.moe_dispatch(t, ids, 8)
+    r, w = rows.detach().requires_grad_(), torch.rand(5, 2, device="cuda", requires_grad=True)
+    for make, leaf in ((lambda: tgo.moe_router(x * 1, 2)[0], x), (lambda: tgo.moe_balance_loss(x * 1, ids)[0], x), (lambda: tgo.moe_dispatch(t * 1, ids, 8)[0], t),
+                       (lambda: tgo.moe_combine(r * 1, at, w), r), (lambda: tgo.moe_combine(r.detach(), at, w * 1), w)):
+        y = make()
+        g = torch.ones_like(y)
+        (a,) = torch.autograd.grad(y, leaf, g, retain_graph=True)
+        (b,) = torch.autograd.grad(y, leaf, g)
+        assert torch.equal(a, b)
+        with pytest.raises(RuntimeError, match="second time"):
+            torch.autograd.grad(y, leaf, g)
+        with torch.autograd.graph.save_on_cpu():
+            z = make()
+        assert torch.equal(torch.autograd.grad(z, leaf, g)[0], a)
+    for change in ("x", "w"):
+        v = x * 1
+        weights, _ = tgo.moe_router(v, 2, normalize=False)
+        total = weights.sum()
+        with torch.no_grad():
+            (v if change == "x" else weights).add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            total.backward()
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x.detach().requires_grad_(), torch.ones_like(x))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            tgo.moe_router(dual, 2)
+    # leaves that share a node with others, and one that wants nothing
+    loss = tgo.moe_combine(tgo.moe_dispatch(t, ids, 8)[0], at, tgo.moe_router(x, 2)[0]).float().sum() + tgo.moe_balance_loss(x, ids)[0]
+    loss.backward()
+    assert x.grad.shape == x.shape and t.grad.shape == t.shape and tgo.moe_router(x.detach(), 2)[0].grad_fn is None
+
+
 def test_compiled_and_checked_by_torch(cuda):
     import torch_ggml_ops_b200 as tgo
 

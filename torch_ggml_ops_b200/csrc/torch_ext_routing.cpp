@@ -5,6 +5,10 @@
 #include <ATen/MemoryOverlap.h>
 
 #include <cstdlib>
+#include <mutex>
+#include <torch/csrc/autograd/FunctionsManual.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 
 #include "torch_ext.h"
 
@@ -43,6 +47,38 @@ std::vector<int64_t> with_last(at::IntArrayRef sizes, int64_t last) {
     std::vector<int64_t> v = sizes.vec();
     v.back() = last;
     return v;
+}
+
+// ------------------------------------------------------------------ formulas
+// As nodes of the graph themselves and not by way of Function, whose context costs some 4 us of a forward and backward pass of 58.
+using torch::autograd::SavedVariable;
+struct Formula : public torch::autograd::Node {
+    using Node::Node;
+    std::vector<SavedVariable> kept;
+    void keep(std::initializer_list<Tensor> inputs) {
+        for (const Tensor& t : inputs) kept.emplace_back(t, false);
+    }
+    variable_list apply(variable_list&& g) override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        variable_list d(num_outputs());
+        if (g[0].defined()) gradients(g[0], d);
+        return d;
+    }
+    void release_variables() override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        for (SavedVariable& v : kept) v.reset_data();
+    }
+    virtual void gradients(const Tensor& g, variable_list& d) = 0;
+};
+// a node whose inputs are `inputs`; an undefined one has no edge
+template <typename N>
+std::shared_ptr<N> formula(std::initializer_list<Tensor> inputs) {
+    torch::autograd::edge_list next;
+    for (const Tensor& t : inputs) {
+        TORCH_CHECK_NOT_IMPLEMENTED(!torch::autograd::isFwGradDefined(t), "forward-mode differentiation of the routing operators is not supported");
+        next.push_back(t.defined() ? torch::autograd::impl::gradient_edge(t) : torch::autograd::Edge());
+    }
+    return std::shared_ptr<N>(new N(std::move(next)), torch::autograd::deleteNode);
 }
 
 // ------------------------------------------------------------------ moe_router
@@ -101,33 +137,33 @@ Tensor call_router_grad(const Tensor& g, const Tensor& x, const Tensor& ids, con
 [[noreturn]] void once_only(const char* name) {
     TORCH_CHECK(false, "torch_ggml_ops_b200::", name, " does not support higher-order gradients");
 }
-struct RouterFn : public Function<RouterFn> {
-    static variable_list forward(AutogradContext* ctx, const Tensor& x, int64_t k, int64_t scoring, bool norm, const std::optional<Tensor>& mask) {
-        at::AutoDispatchBelowADInplaceOrView guard;
-        auto [w, ids] = call_router(x, k, scoring, norm, mask);
-        ctx->save_for_backward({x, ids, w});
-        ctx->saved_data["scoring"] = scoring;
-        ctx->saved_data["norm"] = norm;
-        ctx->mark_non_differentiable({ids});
-        ctx->set_materialize_grads(false);
-        return {w, ids};
+struct RouterFormula : public Formula {
+    using Formula::Formula;
+    int64_t scoring = 0;
+    bool norm = true;
+    void gradients(const Tensor& g, variable_list& d) override {
+        if (task_should_compute_output(0))
+            d[0] = call_router_grad(g, kept[0].unpack(), kept[1].unpack(), kept[2].unpack(shared_from_this()), scoring, norm);
     }
-    static tensor_list backward(AutogradContext* ctx, tensor_list g) {
-        Tensor dx;
-        if (ctx->needs_input_grad(0) && g[0].defined()) {
-            const variable_list s = ctx->get_saved_variables();
-            dx = call_router_grad(g[0], s[0], s[1], s[2], ctx->saved_data["scoring"].toInt(), ctx->saved_data["norm"].toBool());
-        }
-        return {dx, Tensor(), Tensor(), Tensor(), Tensor()};
-    }
+    std::string name() const override { return "MoeRouterBackward"; }
 };
 std::tuple<Tensor, Tensor> router_autograd(const Tensor& x, int64_t k, int64_t scoring, bool norm, const std::optional<Tensor>& mask) {
-    if (wants_grad(x)) {
-        const variable_list r = RouterFn::apply(x, k, scoring, norm, mask);
-        return {r[0], r[1]};
+    if (!wants_grad(x)) {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        return call_router(x, k, scoring, norm, mask);
     }
-    at::AutoDispatchBelowADInplaceOrView guard;
-    return call_router(x, k, scoring, norm, mask);
+    const auto node = formula<RouterFormula>({x});
+    Tensor w, ids;
+    {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        std::tie(w, ids) = call_router(x, k, scoring, norm, mask);
+    }
+    torch::autograd::set_history(w, node);
+    node->keep({x, ids});
+    node->kept.emplace_back(w, true);
+    node->scoring = scoring;
+    node->norm = norm;
+    return {std::move(w), std::move(ids)};
 }
 struct RouterGradFn : public Function<RouterGradFn> {
     static Tensor forward(AutogradContext*, const Tensor& g, const Tensor& x, const Tensor& ids, const Tensor& w, int64_t scoring, bool norm) {
@@ -192,32 +228,29 @@ Tensor call_balance_grad(const Tensor& g, const Tensor& x, const Tensor& ids, co
     static const auto h = op<Tensor(const Tensor&, const Tensor&, const Tensor&, const Tensor&, int64_t)>("torch_ggml_ops_b200::moe_balance_grad");
     return h.call(g, x, ids, coef, scoring);
 }
-struct BalanceFn : public Function<BalanceFn> {
-    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& ids, int64_t scoring) {
-        at::AutoDispatchBelowADInplaceOrView guard;
-        auto [loss, counts, coef] = call_balance(x, ids, scoring);
-        ctx->save_for_backward({x, ids, coef});
-        ctx->saved_data["scoring"] = scoring;
-        ctx->mark_non_differentiable({counts, coef});
-        ctx->set_materialize_grads(false);
-        return {loss, counts, coef};
+struct BalanceFormula : public Formula {
+    using Formula::Formula;
+    int64_t scoring = 0;
+    void gradients(const Tensor& g, variable_list& d) override {
+        if (task_should_compute_output(0)) d[0] = call_balance_grad(g, kept[0].unpack(), kept[1].unpack(), kept[2].unpack(), scoring);
     }
-    static tensor_list backward(AutogradContext* ctx, tensor_list g) {
-        Tensor dx;
-        if (ctx->needs_input_grad(0) && g[0].defined()) {
-            const variable_list s = ctx->get_saved_variables();
-            dx = call_balance_grad(g[0], s[0], s[1], s[2], ctx->saved_data["scoring"].toInt());
-        }
-        return {dx, Tensor(), Tensor()};
-    }
+    std::string name() const override { return "MoeBalanceLossBackward"; }
 };
 std::tuple<Tensor, Tensor, Tensor> balance_autograd(const Tensor& x, const Tensor& ids, int64_t scoring) {
-    if (wants_grad(x)) {
-        const variable_list r = BalanceFn::apply(x, ids, scoring);
-        return {r[0], r[1], r[2]};
+    if (!wants_grad(x)) {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        return call_balance(x, ids, scoring);
     }
-    at::AutoDispatchBelowADInplaceOrView guard;
-    return call_balance(x, ids, scoring);
+    const auto node = formula<BalanceFormula>({x});
+    Tensor loss, counts, coef;
+    {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        std::tie(loss, counts, coef) = call_balance(x, ids, scoring);
+    }
+    torch::autograd::set_history(loss, node);
+    node->keep({x, ids, coef});
+    node->scoring = scoring;
+    return {std::move(loss), std::move(counts), std::move(coef)};
 }
 struct BalanceGradFn : public Function<BalanceGradFn> {
     static Tensor forward(AutogradContext*, const Tensor& g, const Tensor& x, const Tensor& ids, const Tensor& coef, int64_t scoring) {
@@ -327,58 +360,58 @@ std::tuple<Tensor, Tensor> call_combine_grad(const Tensor& g, const Tensor& rows
         "torch_ggml_ops_b200::moe_combine_grad");
     return h.call(g, rows, at_row, w, need_rows, need_weights);
 }
-struct DispatchFn : public Function<DispatchFn> {
-    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& ids, int64_t experts) {
-        at::AutoDispatchBelowADInplaceOrView guard;
-        auto [rows, at_row, indices, offsets] = call_dispatch(x, ids, experts);
-        ctx->save_for_backward({at_row});
-        ctx->mark_non_differentiable({at_row, indices, offsets});
-        ctx->set_materialize_grads(false);
-        return {rows, at_row, indices, offsets};
+struct DispatchFormula : public Formula {
+    using Formula::Formula;
+    void gradients(const Tensor& g, variable_list& d) override {
+        // contiguous rows of a multiple of 8 elements start at 16 bytes in whatever tensor they are a part of
+        if (task_should_compute_output(0)) d[0] = call_combine(g.contiguous(), kept[0].unpack(), std::nullopt);
     }
-    static tensor_list backward(AutogradContext* ctx, tensor_list g) {
-        Tensor dx;
-        if (ctx->needs_input_grad(0) && g[0].defined()) {
-            // contiguous rows of a multiple of 8 elements start at 16 bytes in whatever tensor they are a part of
-            dx = call_combine(g[0].contiguous(), ctx->get_saved_variables()[0], std::nullopt);
-        }
-        return {dx, Tensor(), Tensor()};
-    }
+    std::string name() const override { return "MoeDispatchBackward"; }
 };
 std::tuple<Tensor, Tensor, Tensor, Tensor> dispatch_autograd(const Tensor& x, const Tensor& ids, int64_t experts) {
-    if (wants_grad(x)) {
-        const variable_list r = DispatchFn::apply(x, ids, experts);
-        return {r[0], r[1], r[2], r[3]};
-    }
-    at::AutoDispatchBelowADInplaceOrView guard;
-    return call_dispatch(x, ids, experts);
-}
-struct CombineFn : public Function<CombineFn> {
-    static Tensor forward(AutogradContext* ctx, const Tensor& rows, const Tensor& at_row, const std::optional<Tensor>& w) {
+    if (!wants_grad(x)) {
         at::AutoDispatchBelowADInplaceOrView guard;
-        ctx->save_for_backward({rows, at_row, w.has_value() ? *w : Tensor()});
-        ctx->set_materialize_grads(false);
-        return call_combine(rows, at_row, w);
+        return call_dispatch(x, ids, experts);
     }
-    static tensor_list backward(AutogradContext* ctx, tensor_list g) {
-        Tensor d_rows, d_w;
-        if (g[0].defined()) {
-            const variable_list s = ctx->get_saved_variables();
-            const std::optional<Tensor> w = s[2].defined() ? std::optional<Tensor>(s[2]) : std::nullopt;
-            const bool need_rows = ctx->needs_input_grad(0), need_w = w.has_value() && ctx->needs_input_grad(2);
-            if (need_rows || need_w) {
-                auto [a, b] = call_combine_grad(g[0], s[0], s[1], w, need_rows, need_w);
-                if (need_rows) d_rows = a;
-                if (need_w) d_w = b;
-            }
-        }
-        return {d_rows, Tensor(), d_w};
+    const auto node = formula<DispatchFormula>({x});
+    Tensor rows, at_row, indices, offsets;
+    {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        std::tie(rows, at_row, indices, offsets) = call_dispatch(x, ids, experts);
     }
+    torch::autograd::set_history(rows, node);
+    node->keep({at_row});
+    return {std::move(rows), std::move(at_row), std::move(indices), std::move(offsets)};
+}
+struct CombineFormula : public Formula {
+    using Formula::Formula;
+    bool weighted = false;
+    void gradients(const Tensor& g, variable_list& d) override {
+        const bool need_rows = task_should_compute_output(0), need_w = weighted && task_should_compute_output(1);
+        if (!need_rows && !need_w) return;
+        const std::optional<Tensor> w = weighted ? std::optional<Tensor>(kept[2].unpack()) : std::nullopt;
+        auto [a, b] = call_combine_grad(g, kept[0].unpack(), kept[1].unpack(), w, need_rows, need_w);
+        if (need_rows) d[0] = a;
+        if (need_w) d[1] = b;
+    }
+    std::string name() const override { return "MoeCombineBackward"; }
 };
 Tensor combine_autograd(const Tensor& rows, const Tensor& at_row, const std::optional<Tensor>& w) {
-    if (wants_grad(rows) || (w.has_value() && wants_grad(*w))) return CombineFn::apply(rows, at_row, w);
-    at::AutoDispatchBelowADInplaceOrView guard;
-    return call_combine(rows, at_row, w);
+    if (!wants_grad(rows) && !(w.has_value() && wants_grad(*w))) {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        return call_combine(rows, at_row, w);
+    }
+    const auto node = formula<CombineFormula>({rows, w.has_value() ? *w : Tensor()});
+    Tensor y;
+    {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        y = call_combine(rows, at_row, w);
+    }
+    torch::autograd::set_history(y, node);
+    node->keep({rows, at_row});
+    if (w.has_value()) node->keep({*w});
+    node->weighted = w.has_value();
+    return y;
 }
 struct CombineGradFn : public Function<CombineGradFn> {
     static variable_list forward(AutogradContext*, const Tensor& g, const Tensor& rows, const Tensor& at_row, const std::optional<Tensor>& w, bool need_rows,
