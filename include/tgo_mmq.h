@@ -389,7 +389,7 @@ int tgo_moe_balance_grad(const void* logits, int dtype, int64_t tokens, int64_t 
 /* Token rows x [tokens][width] (bf16, width a multiple of 8) to rows sorted by expert, pairs of one expert in
  * their order: rows [tokens * top_k][width], row_of_pair int32 [tokens][top_k] (-1: the pair's id names no
  * expert), expert_indices / expert_offsets as the grouped calls take them.  Rows behind the last expert's are
- * zeros. */
+ * zeros.  Few pairs need no workspace (0 bytes; null then). */
 int64_t tgo_moe_dispatch_workspace_bytes(int64_t n_pairs, int64_t num_experts);
 int tgo_moe_dispatch(const void* x, const int32_t* expert_ids, int64_t tokens, int64_t top_k, int64_t num_experts, int64_t width,
                      void* rows, int32_t* row_of_pair, int64_t* expert_indices, int32_t* expert_offsets, void* workspace,

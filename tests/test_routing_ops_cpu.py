@@ -45,6 +45,7 @@ def test_the_c_boundary_refuses_before_any_device_work():
         assert call() < 0
         assert needle in native.last_error(), (needle, native.last_error())
     assert lib.tgo_moe_balance_workspace_bytes(0, 8) == -1 and lib.tgo_moe_balance_workspace_bytes(4, 2000) == -1
+    assert lib.tgo_moe_dispatch_workspace_bytes(4096, 8) == 0 < lib.tgo_moe_dispatch_workspace_bytes(4097, 8)
     assert lib.tgo_moe_dispatch_workspace_bytes(-1, 8) == -1 and lib.tgo_moe_dispatch_workspace_bytes(4, 0) == -1
 
 
