@@ -17,7 +17,9 @@
 // while the first runs (16 rows 14.2 to 26, 200 rows fp32 81: its phases are latency, and short histories got slower);
 // clusters of eight blocks that share one reading of the history (all but the longest slower); the history sorted by
 // slices first (a block per row: 5 us and more, as much of a history is in few slices); larger slices with the tables alone in
-// shared memory, looked up in the pass vector by vector (16 rows of 8192 ids, biases and mask 16.9 for 13.8, 200 rows of 16 ids 62 for 42).
+// shared memory, looked up in the pass vector by vector (16 rows of 8192 ids, biases and mask 16.9 for 13.8, 200 rows of 16 ids 62 for 42);
+// the ids of a slice put together by a warp before they are counted (16 rows of 4096 ids 10.1 for 10.7, 200 rows of 16 44 for 42); slices
+// whose number fills the last round of blocks (200 rows of 1500 ids 62 for 58).
 #include "../../include/tgo_mmq.h"
 
 #include <atomic>
