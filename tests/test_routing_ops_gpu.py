@@ -744,3 +744,81 @@ def test_offsets_beyond_32_bits(cuda):
     assert bool((y[-1] == 1.5).all()) and not y[:-1].any()
     (dt,) = torch.autograd.grad(y[-1].sum(), t)
     assert bool((dt[-1] == 1.5).all()) and not dt[:-1].any()
+
+
+def small_step(tgo, logits, tokens):
+    weights, ids = tgo.moe_router(logits, 4, normalize=False)
+    balance, _ = tgo.moe_balance_loss(logits, ids)
+    rows, at, _, _ = tgo.moe_dispatch(tokens, ids, 32)
+    return tgo.moe_combine(rows * 2, at, weights), balance
+
+
+def test_batches_of_any_size_in_one_graph(cuda):
+    import torch_ggml_ops_b200 as tgo
+
+    torch._dynamo.reset()
+    compiled = torch.compile(lambda a, b: small_step(tgo, a, b), dynamic=True, fullgraph=True, backend="aot_eager")
+    for n in (40, 17, 90):
+        a, b = torch.randn(n, 32, device="cuda", requires_grad=True), torch.randn(n, 64, device="cuda").bfloat16().requires_grad_()
+        want, got = small_step(tgo, a, b), compiled(a, b)
+        assert all(torch.equal(p, q) for p, q in zip(want, got))
+        for p, q in zip(*(torch.autograd.grad(y.float().sum() + loss, [a, b]) for y, loss in (want, got))):
+            assert torch.equal(p, q)
+
+
+def test_a_backward_pass_into_leaves_captured(cuda):
+    import torch_ggml_ops_b200 as tgo
+
+    a, b = torch.randn(40, 32, device="cuda", requires_grad=True), torch.randn(40, 64, device="cuda").bfloat16().requires_grad_()
+
+    def step():
+        a.grad = b.grad = None
+        y, loss = small_step(tgo, a, b)
+        (y.float().sum() + loss).backward()
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    want = a.grad.clone(), b.grad.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(a.grad, want[0]) and torch.equal(b.grad, want[1])
+
+
+def test_without_autograd_twice_and_from_several_threads(cuda):
+    import threading
+
+    import torch_ggml_ops_b200 as tgo
+
+    x, t = torch.randn(40, 32, device="cuda"), torch.randn(40, 64, device="cuda").bfloat16()
+    with torch.inference_mode():
+        want = small_step(tgo, x, t)
+    # dispatch is linear: the second derivative of the rows' cubes is 6 x for each of the 4 pairs
+    leaf = t.clone().requires_grad_()
+    ids = tgo.moe_router(x, 4)[1]
+    (g,) = torch.autograd.grad((tgo.moe_dispatch(leaf, ids, 32)[0].float() ** 3).sum(), leaf, create_graph=True)
+    (h,) = torch.autograd.grad(g.float().sum(), leaf)
+    near(h, 24 * t.double(), 2.0 ** -6 * t.double().abs().cpu() * 24)   # two passes, each with two roundings to bf16
+    found = []
+
+    def work():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                y, loss = small_step(tgo, x, t)
+            torch.cuda.current_stream().synchronize()
+            found.append(torch.equal(y, want[0]) and torch.equal(loss, want[1]))
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work) for _ in range(5)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert found == [True] * 5
