@@ -153,9 +153,10 @@ def test_the_same_token_again_and_again(cuda):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,vocab,n_history,n_bias,mask", [(3, 30011, 8150, 42, True), (3, 30011, 8150, 43, False), (2, 100003, 9000, 300, True),
-                                                              (1, 70000, 70000, 0, True), (1, 3000, 66000, 3000, False), (2, 5000, 3, 9000, True)])
+                                                              (1, 70000, 70000, 0, True), (1, 3000, 66000, 3000, False), (2, 5000, 3, 9000, True), (33, 700, 16400, 5, True),
+                                                              (32, 90000, 16384, 0, False), (40, 3, 70000, 1, False)])
 def test_long_histories_and_lists(cuda, dtype, rows, vocab, n_history, n_bias, mask):
-    """Either table of the named tokens, with counts of 16 and 32 bits, in one block and in several."""
+    """Every size of a block, counts of 16 and 32 bits, one slice and several."""
     import torch_ggml_ops_b200 as tgo
 
     c = case(rows, vocab, n_history, n_bias, mask, dtype)
@@ -163,7 +164,7 @@ def test_long_histories_and_lists(cuda, dtype, rows, vocab, n_history, n_bias, m
     d = {k: v.cuda() for k, v in c.items()}
     args = dict(history=d["history"], history_lengths=d["lengths"], repetition_penalty=d["repetition"], presence_penalty=d["presence"],
                 frequency_penalty=d["frequency"], bias_ids=d.get("bias_ids"), bias_values=d.get("bias_values"), allowed=d.get("allowed"))
-    for _ in range(3):
+    for _ in range(2):
         x = d["logits"].clone()
         tgo.logit_rules(x, out=x, **args)
         assert torch.equal(x, got) and torch.equal(tgo.logit_rules(d["logits"], **args), got)

@@ -11,7 +11,7 @@
 // history, from L2, and that is what bounds long ones.  us on one B200 (248320 tokens; in a graph, one call after another):
 //   16 rows bf16 (15.9 MB)      logits alone 4.7, mask 4.8, 16 biases 5.8, 512 ids 7.4, 4096 10.7, 16384 16.2;
 //                               ragged histories up to 8192, biases and mask 13.8
-//   200 rows bf16 (199 MB)      16 ids 42 (4.7 TB/s), 512 50, 4096 65, 16384 122
+//   200 rows bf16 (199 MB)      16 ids 42 (4.7 TB/s), 512 50, 4096 65, 16384 108
 //   200 rows fp32 (397 MB)      logits alone 63.4 (6.3 TB/s, as a copy), mask 65.1, mask and 1500 ids 89
 // Tried: a pass under the mask and a second kernel for the named tokens, with a hash table or ranks in a bit table, that starts
 // while the first runs (16 rows 14.2 to 26, 200 rows fp32 81: its phases are latency, and short histories got slower);
@@ -337,8 +337,9 @@ static int launch_rules(RulesArgs& a, int64_t id_bytes, cudaStream_t st) {
     const bool tables = a.history != nullptr || a.bias_ids != nullptr, narrow = a.history_len <= UINT16_MAX;
     // Every slice reads all of a history, so that of a long one larger slices read less; small ones overlap their phases better
     // (us with 256 / 512 threads, bf16, 248320 tokens: 16 rows of 1024 ids 7.6 / 10.1, of 4096 10.7 / 10.7, of 16384 20.3 / 16.1;
-    // 200 rows of 1024 ids 51.5 / 57.7, of 4096 68.7 / 64.9, of 16384 162 / 122; 1024 threads are slower but for the longest).
-    const int threads = a.history_len < 4096 ? 256 : 512;
+    // 200 rows of 1024 ids 51.5 / 57.7, of 4096 68.7 / 64.9, of 16384 162 / 122; with 512 / 1024: 16 rows of 16384 16.1 / 18.9,
+    // 64 rows 43.6 / 37.2, 200 rows 122 / 108, 64 rows of 8192 29.7 / 33.2).
+    const int threads = a.history_len < 4096 ? 256 : a.history_len < 16384 || a.rows < 32 ? 512 : 1024;
     const int64_t token_bytes = static_cast<int64_t>(sizeof(T)) + (a.history != nullptr ? (narrow ? 2 : 4) : 0) + (a.bias_ids != nullptr ? 4 : 0);
     // the list of named tokens is as long as history and biases together, or as the slice
     const int64_t all_names = a.history_len + a.n_bias, memory = kThreadMemory * threads;
@@ -369,6 +370,7 @@ static int launch_rules(RulesArgs& a, int64_t id_bytes, cudaStream_t st) {
     const int64_t names = all_names < a.slice + kRulesPad ? all_names : a.slice + kRulesPad;
     const size_t smem = static_cast<size_t>(token_bytes) * (a.slice + kRulesPad) + static_cast<size_t>(names) * 2;
     if (threads == 256) return launch_slices<T, uint16_t, 256>(a, smem, st);
+    if (threads == 1024) return narrow ? launch_slices<T, uint16_t, 1024>(a, smem, st) : launch_slices<T, uint32_t, 1024>(a, smem, st);
     return narrow ? launch_slices<T, uint16_t, 512>(a, smem, st) : launch_slices<T, uint32_t, 512>(a, smem, st);
 }
 
