@@ -532,6 +532,47 @@ void rules_out_cuda(const Tensor& logits, const MaybeTensor& history, const Mayb
         if (t->has_value()) at::assert_no_overlap(out, **t);
     rules_into(logits, history, lengths, repetition, repetition_all, presence, presence_all, frequency, frequency_all, bias_ids, bias_values, allowed, out);
 }
+// Neither form has a gradient: what wants one is refused and not dropped.
+void refuse_gradients(std::initializer_list<const Tensor*> tensors, std::initializer_list<const MaybeTensor*> maybe) {
+    const auto check = [](const Tensor& t) {
+        TORCH_CHECK(!wants_grad(t), "logit_rules has no gradient; call it under torch.no_grad() or on detached tensors");
+    };
+    for (const Tensor* t : tensors) check(*t);
+    for (const MaybeTensor* t : maybe)
+        if (t->has_value()) check(**t);
+}
+Tensor rules_autograd(const Tensor& logits, const MaybeTensor& history, const MaybeTensor& lengths, const MaybeTensor& repetition, double repetition_all,
+                      const MaybeTensor& presence, double presence_all, const MaybeTensor& frequency, double frequency_all, const MaybeTensor& bias_ids,
+                      const MaybeTensor& bias_values, const MaybeTensor& allowed) {
+    refuse_gradients({&logits}, {&repetition, &presence, &frequency, &bias_values});
+    static const auto h = op<decltype(rules_cuda)>("torch_ggml_ops_b200::logit_rules");
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return h.call(logits, history, lengths, repetition, repetition_all, presence, presence_all, frequency, frequency_all, bias_ids, bias_values, allowed);
+}
+void call_rules_out(const Tensor& logits, const MaybeTensor& history, const MaybeTensor& lengths, const MaybeTensor& repetition, double repetition_all,
+                    const MaybeTensor& presence, double presence_all, const MaybeTensor& frequency, double frequency_all, const MaybeTensor& bias_ids,
+                    const MaybeTensor& bias_values, const MaybeTensor& allowed, Tensor& out) {
+    static const auto h = op<decltype(rules_out_cuda)>("torch_ggml_ops_b200::logit_rules_out");
+    h.call(logits, history, lengths, repetition, repetition_all, presence, presence_all, frequency, frequency_all, bias_ids, bias_values, allowed, out);
+}
+void rules_out_autograd(const Tensor& logits, const MaybeTensor& history, const MaybeTensor& lengths, const MaybeTensor& repetition, double repetition_all,
+                        const MaybeTensor& presence, double presence_all, const MaybeTensor& frequency, double frequency_all, const MaybeTensor& bias_ids,
+                        const MaybeTensor& bias_values, const MaybeTensor& allowed, Tensor& out) {
+    refuse_gradients({&logits, &out}, {&repetition, &presence, &frequency, &bias_values});
+    at::AutoDispatchBelowAutograd guard;
+    call_rules_out(logits, history, lengths, repetition, repetition_all, presence, presence_all, frequency, frequency_all, bias_ids, bias_values, allowed, out);
+}
+// Whoever kept out for a backward pass learns from its version that it was written over.  (A tensor of inference mode has no
+// version, as nothing keeps it.)
+void rules_out_versioned(const Tensor& logits, const MaybeTensor& history, const MaybeTensor& lengths, const MaybeTensor& repetition, double repetition_all,
+                         const MaybeTensor& presence, double presence_all, const MaybeTensor& frequency, double frequency_all, const MaybeTensor& bias_ids,
+                         const MaybeTensor& bias_values, const MaybeTensor& allowed, Tensor& out) {
+    {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        call_rules_out(logits, history, lengths, repetition, repetition_all, presence, presence_all, frequency, frequency_all, bias_ids, bias_values, allowed, out);
+    }
+    if (!out.is_inference()) torch::autograd::impl::bump_version(out);
+}
 
 }  // namespace
 
@@ -569,4 +610,7 @@ TORCH_LIBRARY_IMPL(torch_ggml_ops_b200, Autograd, m) {
     m.impl("moe_dispatch", &dispatch_autograd);
     m.impl("moe_combine", &combine_autograd);
     m.impl("moe_combine_grad", &combine_grad_autograd);
+    m.impl("logit_rules", &rules_autograd);
+    m.impl("logit_rules_out", &rules_out_autograd);
 }
+TORCH_LIBRARY_IMPL(torch_ggml_ops_b200, ADInplaceOrView, m) { m.impl("logit_rules_out", &rules_out_versioned); }

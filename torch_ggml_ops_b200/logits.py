@@ -37,9 +37,7 @@ def logit_rules(logits: torch.Tensor, *, history: torch.Tensor | None = None, hi
     apart.  Ids outside the vocabulary name nothing (pad with -1).  A row whose mask leaves no token is -inf throughout.
 
     Returns a new tensor like ``logits``, or writes ``out``, which may be ``logits`` itself: then only what changes is
-    written.  For generation: no gradient."""
-    if torch.is_grad_enabled() and logits.requires_grad:
-        raise RuntimeError("logit_rules has no gradient; call it under torch.no_grad() or on logits.detach()")
+    written.  For generation: no gradient, and tensors that want one are refused."""
     rep, rep_all = (repetition_penalty, 1.0) if isinstance(repetition_penalty, torch.Tensor) else (None, repetition_penalty)
     pres, pres_all = (presence_penalty, 0.0) if isinstance(presence_penalty, torch.Tensor) else (None, presence_penalty)
     freq, freq_all = (frequency_penalty, 0.0) if isinstance(frequency_penalty, torch.Tensor) else (None, frequency_penalty)
