@@ -174,7 +174,7 @@ struct PairDxFn : public Function<PairDxFn> {
     static tensor_list backward(AutogradContext*, tensor_list) { no_second_order("grouped_mmq_pair_grad_input"); }
 };
 Tensor pair_dx_autograd(const Tensor& d0, const Tensor& d1, const Tensor& w0, const Tensor& w1, const Tensor& ei, const Tensor& eo, int64_t qt, int64_t k) {
-    if (wants_grad(d0) || wants_grad(d1)) return PairDxFn::apply(d0, d1, w0, w1, ei, eo, qt, k);
+    if (wants_grad(d0, d1)) return PairDxFn::apply(d0, d1, w0, w1, ei, eo, qt, k);
     at::AutoDispatchBelowADInplaceOrView guard;
     return call_pair_dx(d0, d1, w0, w1, ei, eo, qt, k);
 }
@@ -301,7 +301,7 @@ struct SwigluFn : public Function<SwigluFn> {
     }
 };
 Tensor swiglu_autograd(const Tensor& g, const Tensor& u) {
-    if (wants_grad(g) || wants_grad(u)) return SwigluFn::apply(g, u);
+    if (wants_grad(g, u)) return SwigluFn::apply(g, u);
     at::AutoDispatchBelowADInplaceOrView guard;
     return call_swiglu(g, u);
 }
@@ -318,7 +318,7 @@ struct SwigluGradFn : public Function<SwigluGradFn> {
     }
 };
 std::tuple<Tensor, Tensor> swiglu_grad_autograd(const Tensor& d, const Tensor& g, const Tensor& u) {
-    if (wants_grad(d) || wants_grad(g) || wants_grad(u)) {
+    if (wants_grad(d, g, u)) {
         const variable_list r = SwigluGradFn::apply(d, g, u);
         return {r[0], r[1]};
     }

@@ -23,7 +23,17 @@ template <typename Fn>
 const c10::TypedOperatorHandle<Fn> op(const char* name) {
     return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Fn>();
 }
-inline bool wants_grad(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+// Whether one of an operator's differentiable inputs wants a gradient.  No operator here has a forward-mode derivative: a tangent is
+// refused, on whichever input it is, because the way below autograd would drop it and answer with a derivative of zero.
+inline bool one_wants_grad(const Tensor& t) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), "torch_ggml_ops operators do not support forward-mode differentiation");
+    return t.requires_grad();
+}
+inline bool one_wants_grad(const std::optional<Tensor>& t) { return t.has_value() && one_wants_grad(*t); }
+template <typename... T>
+bool wants_grad(const T&... t) {
+    return (... | one_wants_grad(t)) && at::GradMode::is_enabled();
+}
 inline void check_rc(int rc, const char* what) { TORCH_CHECK(rc == TGO_OK, what, " failed: ", tgo_last_error()); }
 inline void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 

@@ -6,7 +6,6 @@
 
 #include <cstdlib>
 #include <mutex>
-#include <torch/csrc/autograd/FunctionsManual.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 
@@ -74,10 +73,7 @@ struct Formula : public torch::autograd::Node {
 template <typename N>
 std::shared_ptr<N> formula(std::initializer_list<Tensor> inputs) {
     torch::autograd::edge_list next;
-    for (const Tensor& t : inputs) {
-        TORCH_CHECK_NOT_IMPLEMENTED(!torch::autograd::isFwGradDefined(t), "forward-mode differentiation of the routing operators is not supported");
-        next.push_back(t.defined() ? torch::autograd::impl::gradient_edge(t) : torch::autograd::Edge());
-    }
+    for (const Tensor& t : inputs) next.push_back(t.defined() ? torch::autograd::impl::gradient_edge(t) : torch::autograd::Edge());
     return std::shared_ptr<N>(new N(std::move(next)), torch::autograd::deleteNode);
 }
 
@@ -173,7 +169,7 @@ struct RouterGradFn : public Function<RouterGradFn> {
     static tensor_list backward(AutogradContext*, tensor_list) { once_only("moe_router_grad"); }
 };
 Tensor router_grad_autograd(const Tensor& g, const Tensor& x, const Tensor& ids, const Tensor& w, int64_t scoring, bool norm) {
-    if (wants_grad(g) || wants_grad(x) || wants_grad(w)) return RouterGradFn::apply(g, x, ids, w, scoring, norm);
+    if (wants_grad(g, x, w)) return RouterGradFn::apply(g, x, ids, w, scoring, norm);
     at::AutoDispatchBelowADInplaceOrView guard;
     return call_router_grad(g, x, ids, w, scoring, norm);
 }
@@ -260,7 +256,7 @@ struct BalanceGradFn : public Function<BalanceGradFn> {
     static tensor_list backward(AutogradContext*, tensor_list) { once_only("moe_balance_grad"); }
 };
 Tensor balance_grad_autograd(const Tensor& g, const Tensor& x, const Tensor& ids, const Tensor& coef, int64_t scoring) {
-    if (wants_grad(g) || wants_grad(x)) return BalanceGradFn::apply(g, x, ids, coef, scoring);
+    if (wants_grad(g, x, coef)) return BalanceGradFn::apply(g, x, ids, coef, scoring);
     at::AutoDispatchBelowADInplaceOrView guard;
     return call_balance_grad(g, x, ids, coef, scoring);
 }
@@ -397,7 +393,7 @@ struct CombineFormula : public Formula {
     std::string name() const override { return "MoeCombineBackward"; }
 };
 Tensor combine_autograd(const Tensor& rows, const Tensor& at_row, const std::optional<Tensor>& w) {
-    if (!wants_grad(rows) && !(w.has_value() && wants_grad(*w))) {
+    if (!wants_grad(rows, w)) {
         at::AutoDispatchBelowADInplaceOrView guard;
         return call_combine(rows, at_row, w);
     }
@@ -424,7 +420,7 @@ struct CombineGradFn : public Function<CombineGradFn> {
 };
 std::tuple<Tensor, Tensor> combine_grad_autograd(const Tensor& g, const Tensor& rows, const Tensor& at_row, const std::optional<Tensor>& w, bool need_rows,
                                                  bool need_weights) {
-    if (wants_grad(g) || wants_grad(rows) || (w.has_value() && wants_grad(*w))) {
+    if (wants_grad(g, rows, w)) {
         const variable_list r = CombineGradFn::apply(g, rows, at_row, w, need_rows, need_weights);
         return {r[0], r[1]};
     }
@@ -533,18 +529,14 @@ void rules_out_cuda(const Tensor& logits, const MaybeTensor& history, const Mayb
     rules_into(logits, history, lengths, repetition, repetition_all, presence, presence_all, frequency, frequency_all, bias_ids, bias_values, allowed, out);
 }
 // Neither form has a gradient: what wants one is refused and not dropped.
-void refuse_gradients(std::initializer_list<const Tensor*> tensors, std::initializer_list<const MaybeTensor*> maybe) {
-    const auto check = [](const Tensor& t) {
-        TORCH_CHECK(!wants_grad(t), "logit_rules has no gradient; call it under torch.no_grad() or on detached tensors");
-    };
-    for (const Tensor* t : tensors) check(*t);
-    for (const MaybeTensor* t : maybe)
-        if (t->has_value()) check(**t);
+template <typename... T>
+void refuse_gradients(const T&... t) {
+    TORCH_CHECK(!wants_grad(t...), "logit_rules has no gradient; call it under torch.no_grad() or on detached tensors");
 }
 Tensor rules_autograd(const Tensor& logits, const MaybeTensor& history, const MaybeTensor& lengths, const MaybeTensor& repetition, double repetition_all,
                       const MaybeTensor& presence, double presence_all, const MaybeTensor& frequency, double frequency_all, const MaybeTensor& bias_ids,
                       const MaybeTensor& bias_values, const MaybeTensor& allowed) {
-    refuse_gradients({&logits}, {&repetition, &presence, &frequency, &bias_values});
+    refuse_gradients(logits, repetition, presence, frequency, bias_values);
     static const auto h = op<decltype(rules_cuda)>("torch_ggml_ops_b200::logit_rules");
     at::AutoDispatchBelowADInplaceOrView guard;
     return h.call(logits, history, lengths, repetition, repetition_all, presence, presence_all, frequency, frequency_all, bias_ids, bias_values, allowed);
@@ -558,7 +550,7 @@ void call_rules_out(const Tensor& logits, const MaybeTensor& history, const Mayb
 void rules_out_autograd(const Tensor& logits, const MaybeTensor& history, const MaybeTensor& lengths, const MaybeTensor& repetition, double repetition_all,
                         const MaybeTensor& presence, double presence_all, const MaybeTensor& frequency, double frequency_all, const MaybeTensor& bias_ids,
                         const MaybeTensor& bias_values, const MaybeTensor& allowed, Tensor& out) {
-    refuse_gradients({&logits, &out}, {&repetition, &presence, &frequency, &bias_values});
+    refuse_gradients(logits, out, repetition, presence, frequency, bias_values);
     at::AutoDispatchBelowAutograd guard;
     call_rules_out(logits, history, lengths, repetition, repetition_all, presence, presence_all, frequency, frequency_all, bias_ids, bias_values, allowed, out);
 }
