@@ -3,11 +3,13 @@
 // (moe_router, moe_balance_loss, moe_dispatch, moe_combine, with their gradients) and the rules on a
 // generation step's logits (logit_rules).
 #include <ATen/MemoryOverlap.h>
+#include <c10/util/ScopeExit.h>
 
 #include <cstdlib>
 #include <mutex>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/dynamo/compiled_autograd.h>
 
 #include "torch_ext.h"
 
@@ -54,6 +56,9 @@ using torch::autograd::SavedVariable;
 struct Formula : public torch::autograd::Node {
     using Node::Node;
     std::vector<SavedVariable> kept;
+    SavedVariable result;             // the node's own, where a formula needs it
+    int64_t scoring = 0;
+    bool norm = true, weighted = false;
     void keep(std::initializer_list<Tensor> inputs) {
         for (const Tensor& t : inputs) kept.emplace_back(t, false);
     }
@@ -66,6 +71,24 @@ struct Formula : public torch::autograd::Node {
     void release_variables() override {
         const std::lock_guard<std::mutex> lock(mutex_);
         for (SavedVariable& v : kept) v.reset_data();
+        result.reset_data();
+    }
+    // for compiled autograd: what is kept, what a traced graph is specialised on, and the formula with traced tensors in the place of the kept ones
+    void compiled_args(torch::dynamo::autograd::CompiledNodeArgs& args) const override {
+        args.collect(kept, false);
+        args.collect(result, true);
+        args.collect(scoring);
+        args.collect(norm);
+        args.collect(weighted);
+    }
+    variable_list apply_with_saved(const variable_list& inputs, torch::dynamo::autograd::SwapSavedVariables& saved) override {
+        saved.before(kept);
+        saved.before(result);
+        const auto back = c10::make_scope_exit([&] {
+            saved.after(kept);
+            saved.after(result);
+        });
+        return apply(variable_list(inputs));
     }
     virtual void gradients(const Tensor& g, variable_list& d) = 0;
 };
@@ -135,11 +158,9 @@ Tensor call_router_grad(const Tensor& g, const Tensor& x, const Tensor& ids, con
 }
 struct RouterFormula : public Formula {
     using Formula::Formula;
-    int64_t scoring = 0;
-    bool norm = true;
     void gradients(const Tensor& g, variable_list& d) override {
         if (task_should_compute_output(0))
-            d[0] = call_router_grad(g, kept[0].unpack(), kept[1].unpack(), kept[2].unpack(shared_from_this()), scoring, norm);
+            d[0] = call_router_grad(g, kept[0].unpack(), kept[1].unpack(), result.unpack(shared_from_this()), scoring, norm);
     }
     std::string name() const override { return "MoeRouterBackward"; }
 };
@@ -156,7 +177,7 @@ std::tuple<Tensor, Tensor> router_autograd(const Tensor& x, int64_t k, int64_t s
     }
     torch::autograd::set_history(w, node);
     node->keep({x, ids});
-    node->kept.emplace_back(w, true);
+    node->result = SavedVariable(w, true);
     node->scoring = scoring;
     node->norm = norm;
     return {std::move(w), std::move(ids)};
@@ -226,7 +247,6 @@ Tensor call_balance_grad(const Tensor& g, const Tensor& x, const Tensor& ids, co
 }
 struct BalanceFormula : public Formula {
     using Formula::Formula;
-    int64_t scoring = 0;
     void gradients(const Tensor& g, variable_list& d) override {
         if (task_should_compute_output(0)) d[0] = call_balance_grad(g, kept[0].unpack(), kept[1].unpack(), kept[2].unpack(), scoring);
     }
@@ -381,7 +401,6 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> dispatch_autograd(const Tensor& x, co
 }
 struct CombineFormula : public Formula {
     using Formula::Formula;
-    bool weighted = false;
     void gradients(const Tensor& g, variable_list& d) override {
         const bool need_rows = task_should_compute_output(0), need_w = weighted && task_should_compute_output(1);
         if (!need_rows && !need_w) return;
