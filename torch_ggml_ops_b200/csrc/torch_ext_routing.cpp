@@ -58,7 +58,8 @@ struct Formula : public torch::autograd::Node {
     std::vector<SavedVariable> kept;
     SavedVariable result;             // the node's own, where a formula needs it
     int64_t scoring = 0;
-    bool norm = true, weighted = false;
+    bool norm = true;
+    c10::SymInt rows = 0;             // a size that a formula needs of an input that it does not keep
     void keep(std::initializer_list<Tensor> inputs) {
         for (const Tensor& t : inputs) kept.emplace_back(t, false);
     }
@@ -79,14 +80,16 @@ struct Formula : public torch::autograd::Node {
         args.collect(result, true);
         args.collect(scoring);
         args.collect(norm);
-        args.collect(weighted);
+        args.collect(rows);
     }
     variable_list apply_with_saved(const variable_list& inputs, torch::dynamo::autograd::SwapSavedVariables& saved) override {
         saved.before(kept);
         saved.before(result);
+        saved.before(rows);
         const auto back = c10::make_scope_exit([&] {
             saved.after(kept);
             saved.after(result);
+            saved.after(rows);
         });
         return apply(variable_list(inputs));
     }
@@ -313,17 +316,20 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> dispatch_cuda(const Tensor& x, const 
              "moe_dispatch");
     return {rows, at_row, indices, offsets};
 }
+void check_map(const Tensor& at_row, const std::optional<Tensor>& w, const Tensor& like) {
+    check_plain(at_row, like, at::kInt, "row_of_pair");
+    TORCH_CHECK(at_row.dim() >= 1, "row_of_pair must have shape [..., top_k]");
+    check_pairs(at_row.numel(), at_row.size(-1));
+    if (w.has_value()) {
+        check_plain(*w, like, at::kFloat, "weights");
+        TORCH_CHECK(w->sizes() == at_row.sizes(), "weights must have one entry per pair");
+    }
+}
 void check_combine(const Tensor& rows, const Tensor& at_row, const std::optional<Tensor>& w) {
     check_moved(rows, "rows");
     TORCH_CHECK(rows.dim() == 2, "rows must have shape [rows, width]");
     TORCH_CHECK(rows.size(0) <= INT32_MAX, "too many rows");
-    check_plain(at_row, rows, at::kInt, "row_of_pair");
-    TORCH_CHECK(at_row.dim() >= 1, "row_of_pair must have shape [..., top_k]");
-    check_pairs(at_row.numel(), at_row.size(-1));
-    if (w.has_value()) {
-        check_plain(*w, rows, at::kFloat, "weights");
-        TORCH_CHECK(w->sizes() == at_row.sizes(), "weights must have one entry per pair");
-    }
+    check_map(at_row, w, rows);
 }
 Tensor combine_cuda(const Tensor& rows, const Tensor& at_row, const std::optional<Tensor>& w) {
     check_combine(rows, at_row, w);
@@ -338,29 +344,49 @@ Tensor combine_cuda(const Tensor& rows, const Tensor& at_row, const std::optiona
                  "moe_combine");
     return out;
 }
+// The gradients of combine: of `rows` where n_rows is no less than 0, of the weights where `rows` are there.
+std::tuple<Tensor, Tensor> combine_grads(const Tensor& grad, const std::optional<Tensor>& rows, int64_t n_rows, const Tensor& at_row,
+                                         const std::optional<Tensor>& w) {
+    const int64_t h = grad.size(-1), k = at_row.size(-1), tokens = at_row.numel() / k;
+    const bool need_rows = n_rows >= 0, need_weights = rows.has_value();
+    Tensor d = grad.contiguous();
+    if (reinterpret_cast<uintptr_t>(d.const_data_ptr()) % 16 != 0) d = d.clone();
+    Tensor d_rows = new_cuda({need_rows ? n_rows : 0, h}, at::kBFloat16, grad);
+    Tensor d_w = need_weights ? new_cuda(at_row.sizes(), at::kFloat, grad) : new_cuda({0}, at::kFloat, grad);
+    if (!need_rows && !need_weights) return {d_rows, d_w};
+    const int64_t existing = need_weights ? rows->size(0) : n_rows;
+    if (existing == 0 || tokens == 0) return {d_rows.zero_(), d_w.zero_()};
+    const int64_t bytes = need_rows ? n_rows * 4 : 0;
+    const Tensor ws = bytes > 0 ? new_cuda({bytes}, at::kByte, grad) : Tensor();
+    check_rc(tgo_moe_combine_grad(d.const_data_ptr(), need_weights ? rows->const_data_ptr() : nullptr, existing, at_row.const_data_ptr<int32_t>(),
+                                  w.has_value() ? w->const_data_ptr<float>() : nullptr, need_rows ? d_rows.mutable_data_ptr() : nullptr,
+                                  need_weights ? d_w.mutable_data_ptr<float>() : nullptr, tokens, k, h, bytes > 0 ? ws.mutable_data_ptr() : nullptr,
+                                  bytes, stream_of(grad)),
+             "moe_combine_grad");
+    return {d_rows, d_w};
+}
+void check_result_grad(const Tensor& grad, const Tensor& at_row) {
+    TORCH_CHECK(grad.is_cuda() && grad.device() == at_row.device() && grad.scalar_type() == at::kBFloat16 && grad.dim() == at_row.dim() &&
+                    grad.sizes().slice(0, grad.dim() - 1) == at_row.sizes().slice(0, grad.dim() - 1),
+                "grad must be a torch.bfloat16 tensor like the result");
+}
 // an empty tensor in the place of a gradient that is not wanted
 std::tuple<Tensor, Tensor> combine_grad_cuda(const Tensor& grad, const Tensor& rows, const Tensor& at_row, const std::optional<Tensor>& w, bool need_rows,
                                              bool need_weights) {
     check_combine(rows, at_row, w);
-    const int64_t h = rows.size(1), k = at_row.size(-1), tokens = at_row.numel() / k;
+    check_result_grad(grad, at_row);
+    TORCH_CHECK(grad.size(-1) == rows.size(1), "grad must be a torch.bfloat16 tensor like the result");
     const c10::cuda::CUDAGuard guard(rows.device());
-    TORCH_CHECK(grad.device() == rows.device() && grad.scalar_type() == at::kBFloat16 && grad.dim() == at_row.dim() && grad.size(-1) == h &&
-                    grad.numel() == tokens * h,
-                "grad must be a torch.bfloat16 tensor like the result");
-    Tensor d = grad.contiguous();
-    if (reinterpret_cast<uintptr_t>(d.const_data_ptr()) % 16 != 0) d = d.clone();
-    Tensor d_rows = new_cuda({need_rows ? rows.size(0) : 0, h}, at::kBFloat16, rows);
-    Tensor d_w = need_weights ? new_cuda(at_row.sizes(), at::kFloat, rows) : new_cuda({0}, at::kFloat, rows);
-    if (rows.size(0) == 0 || tokens == 0) return {d_rows.zero_(), d_w.zero_()};
-    if (!need_rows && !need_weights) return {d_rows, d_w};
-    const int64_t bytes = need_rows ? rows.size(0) * 4 : 0;
-    const Tensor ws = bytes > 0 ? new_cuda({bytes}, at::kByte, rows) : Tensor();
-    check_rc(tgo_moe_combine_grad(d.const_data_ptr(), rows.const_data_ptr(), rows.size(0), at_row.const_data_ptr<int32_t>(),
-                                  w.has_value() ? w->const_data_ptr<float>() : nullptr, need_rows ? d_rows.mutable_data_ptr() : nullptr,
-                                  need_weights ? d_w.mutable_data_ptr<float>() : nullptr, tokens, k, h, bytes > 0 ? ws.mutable_data_ptr() : nullptr,
-                                  bytes, stream_of(rows)),
-             "moe_combine_grad");
-    return {d_rows, d_w};
+    return combine_grads(grad, need_weights ? std::optional<Tensor>(rows) : std::nullopt, need_rows ? rows.size(0) : -1, at_row, w);
+}
+// the gradient of the rows alone, for which the rows themselves are not needed
+Tensor combine_rows_grad_cuda(const Tensor& grad, const Tensor& at_row, const std::optional<Tensor>& w, int64_t n_rows) {
+    TORCH_CHECK(n_rows >= 0 && n_rows <= INT32_MAX, "the number of rows must be in 0..2^31-1; got ", n_rows);
+    check_map(at_row, w, grad);
+    check_result_grad(grad, at_row);
+    TORCH_CHECK(grad.size(-1) > 0 && grad.size(-1) % 8 == 0, "grad must have rows whose length is a positive multiple of 8");
+    const c10::cuda::CUDAGuard guard(grad.device());
+    return std::get<0>(combine_grads(grad, std::nullopt, n_rows, at_row, w));
 }
 std::tuple<Tensor, Tensor, Tensor, Tensor> call_dispatch(const Tensor& x, const Tensor& ids, int64_t experts) {
     static const auto h = op<std::tuple<Tensor, Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, int64_t)>("torch_ggml_ops_b200::moe_dispatch");
@@ -375,6 +401,10 @@ std::tuple<Tensor, Tensor> call_combine_grad(const Tensor& g, const Tensor& rows
     static const auto h = op<std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const std::optional<Tensor>&, bool, bool)>(
         "torch_ggml_ops_b200::moe_combine_grad");
     return h.call(g, rows, at_row, w, need_rows, need_weights);
+}
+Tensor call_combine_rows_grad(const Tensor& g, const Tensor& at_row, const std::optional<Tensor>& w, c10::SymInt n_rows) {
+    static const auto h = op<Tensor(const Tensor&, const Tensor&, const std::optional<Tensor>&, c10::SymInt)>("torch_ggml_ops_b200::moe_combine_rows_grad");
+    return h.call(g, at_row, w, std::move(n_rows));
 }
 struct DispatchFormula : public Formula {
     using Formula::Formula;
@@ -399,13 +429,20 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> dispatch_autograd(const Tensor& x, co
     node->keep({at_row});
     return {std::move(rows), std::move(at_row), std::move(indices), std::move(offsets)};
 }
+// Keeps the map; the weights, where the rows want a gradient; the rows, where the weights do.  What is kept is handed on, needed for the gradients
+// asked for or not: compiled autograd wants a use of all that it unpacks.
 struct CombineFormula : public Formula {
     using Formula::Formula;
     void gradients(const Tensor& g, variable_list& d) override {
-        const bool need_rows = task_should_compute_output(0), need_w = weighted && task_should_compute_output(1);
+        const bool need_rows = task_should_compute_output(0), need_w = task_should_compute_output(1);
         if (!need_rows && !need_w) return;
-        const std::optional<Tensor> w = weighted ? std::optional<Tensor>(kept[2].unpack()) : std::nullopt;
-        auto [a, b] = call_combine_grad(g, kept[0].unpack(), kept[1].unpack(), w, need_rows, need_w);
+        const Tensor at_row = kept[0].unpack(), kept_w = kept[1].unpack(), kept_rows = kept[2].unpack();
+        const std::optional<Tensor> w = kept_w.defined() ? std::optional<Tensor>(kept_w) : std::nullopt;
+        if (!kept_rows.defined()) {
+            d[0] = call_combine_rows_grad(g, at_row, w, rows);
+            return;
+        }
+        auto [a, b] = call_combine_grad(g, kept_rows, at_row, w, need_rows, need_w);
         if (need_rows) d[0] = a;
         if (need_w) d[1] = b;
     }
@@ -416,6 +453,7 @@ Tensor combine_autograd(const Tensor& rows, const Tensor& at_row, const std::opt
         at::AutoDispatchBelowADInplaceOrView guard;
         return call_combine(rows, at_row, w);
     }
+    const bool of_weights = w.has_value() && w->requires_grad();
     const auto node = formula<CombineFormula>({rows, w.has_value() ? *w : Tensor()});
     Tensor y;
     {
@@ -423,9 +461,8 @@ Tensor combine_autograd(const Tensor& rows, const Tensor& at_row, const std::opt
         y = call_combine(rows, at_row, w);
     }
     torch::autograd::set_history(y, node);
-    node->keep({rows, at_row});
-    if (w.has_value()) node->keep({*w});
-    node->weighted = w.has_value();
+    node->keep({at_row, w.has_value() && rows.requires_grad() ? *w : Tensor(), of_weights ? rows : Tensor()});
+    node->rows = rows.sym_size(0);
     return y;
 }
 struct CombineGradFn : public Function<CombineGradFn> {
@@ -445,6 +482,19 @@ std::tuple<Tensor, Tensor> combine_grad_autograd(const Tensor& g, const Tensor& 
     }
     at::AutoDispatchBelowADInplaceOrView guard;
     return call_combine_grad(g, rows, at_row, w, need_rows, need_weights);
+}
+
+struct CombineRowsGradFn : public Function<CombineRowsGradFn> {
+    static Tensor forward(AutogradContext*, const Tensor& g, const Tensor& at_row, const std::optional<Tensor>& w, c10::SymInt n_rows) {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        return call_combine_rows_grad(g, at_row, w, std::move(n_rows));
+    }
+    static tensor_list backward(AutogradContext*, tensor_list) { once_only("moe_combine_rows_grad"); }
+};
+Tensor combine_rows_grad_autograd(const Tensor& g, const Tensor& at_row, const std::optional<Tensor>& w, c10::SymInt n_rows) {
+    if (wants_grad(g, w)) return CombineRowsGradFn::apply(g, at_row, w, std::move(n_rows));
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return call_combine_rows_grad(g, at_row, w, std::move(n_rows));
 }
 
 // ------------------------------------------------------------------ logit_rules
@@ -595,6 +645,7 @@ TORCH_LIBRARY_FRAGMENT(torch_ggml_ops_b200, m) {
     m.def("moe_dispatch(Tensor input, Tensor expert_ids, int num_experts) -> (Tensor, Tensor, Tensor, Tensor)");
     m.def("moe_combine(Tensor rows, Tensor row_of_pair, Tensor? weights) -> Tensor");
     m.def("moe_combine_grad(Tensor grad, Tensor rows, Tensor row_of_pair, Tensor? weights, bool need_rows, bool need_weights) -> (Tensor, Tensor)");
+    m.def("moe_combine_rows_grad(Tensor grad, Tensor row_of_pair, Tensor? weights, SymInt n_rows) -> Tensor");
     m.def(
         "logit_rules(Tensor logits, Tensor? history, Tensor? history_lengths, Tensor? repetition, float repetition_all, Tensor? presence, "
         "float presence_all, Tensor? frequency, float frequency_all, Tensor? bias_ids, Tensor? bias_values, Tensor? allowed) -> Tensor");
@@ -610,6 +661,7 @@ TORCH_LIBRARY_IMPL(torch_ggml_ops_b200, CUDA, m) {
     m.impl("moe_dispatch", &dispatch_cuda);
     m.impl("moe_combine", &combine_cuda);
     m.impl("moe_combine_grad", &combine_grad_cuda);
+    m.impl("moe_combine_rows_grad", &combine_rows_grad_cuda);
     m.impl("logit_rules", &rules_cuda);
     m.impl("logit_rules_out", &rules_out_cuda);
 }
@@ -621,6 +673,7 @@ TORCH_LIBRARY_IMPL(torch_ggml_ops_b200, Autograd, m) {
     m.impl("moe_dispatch", &dispatch_autograd);
     m.impl("moe_combine", &combine_autograd);
     m.impl("moe_combine_grad", &combine_grad_autograd);
+    m.impl("moe_combine_rows_grad", &combine_rows_grad_autograd);
     m.impl("logit_rules", &rules_autograd);
     m.impl("logit_rules_out", &rules_out_autograd);
 }

@@ -62,6 +62,11 @@ def _(grad, rows, row_of_pair, weights, need_rows, need_weights):
             rows.new_empty(row_of_pair.shape if need_weights else (0,), dtype=torch.float32))
 
 
+@torch.library.register_fake(f"{_NS}::moe_combine_rows_grad")
+def _(grad, row_of_pair, weights, n_rows):
+    return grad.new_empty((n_rows, grad.shape[-1]))
+
+
 def _scoring(name: str) -> int:
     try:
         return SCORINGS[name]
@@ -115,7 +120,8 @@ def moe_combine(rows: torch.Tensor, row_of_pair: torch.Tensor, weights: torch.Te
     it, ``weights`` fp32 of the same shape (None: 1).  Pairs whose row is not in ``rows`` add nothing.
 
     Differentiable with respect to ``rows`` and ``weights``, once (a row that no pair names gets a gradient of
-    zeros, one that several name their sum)."""
+    zeros, one that several name their sum).  Only a gradient of the weights needs ``rows`` again: without one they are
+    not kept for the backward pass and may be written over."""
     return _ops.moe_combine.default(rows, row_of_pair, weights)
 
 
