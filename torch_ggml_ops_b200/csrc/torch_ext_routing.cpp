@@ -331,8 +331,7 @@ void check_combine(const Tensor& rows, const Tensor& at_row, const std::optional
     TORCH_CHECK(rows.size(0) <= INT32_MAX, "too many rows");
     check_map(at_row, w, rows);
 }
-Tensor combine_cuda(const Tensor& rows, const Tensor& at_row, const std::optional<Tensor>& w) {
-    check_combine(rows, at_row, w);
+Tensor combine_run(const Tensor& rows, const Tensor& at_row, const std::optional<Tensor>& w) {
     const int64_t h = rows.size(1), k = at_row.size(-1), tokens = at_row.numel() / k;
     const c10::cuda::CUDAGuard guard(rows.device());
     const auto sizes = with_last(at_row.sizes(), h);
@@ -344,13 +343,29 @@ Tensor combine_cuda(const Tensor& rows, const Tensor& at_row, const std::optiona
                  "moe_combine");
     return out;
 }
+Tensor combine_cuda(const Tensor& rows, const Tensor& at_row, const std::optional<Tensor>& w) {
+    check_combine(rows, at_row, w);
+    return combine_run(rows, at_row, w);
+}
+// A cotangent is what autograd makes of it: a view of a larger tensor that starts anywhere, or no plain rows at all.
+Tensor plain_rows(const Tensor& grad) {
+    const Tensor d = grad.contiguous();
+    return reinterpret_cast<uintptr_t>(d.const_data_ptr()) % 16 == 0 ? d : d.clone();
+}
+// the gradient of dispatch: a token's sum over its pairs' rows
+Tensor dispatch_grad_cuda(const Tensor& grad, const Tensor& at_row) {
+    TORCH_CHECK(grad.is_cuda() && grad.scalar_type() == at::kBFloat16 && grad.dim() == 2 && grad.size(1) > 0 && grad.size(1) % 8 == 0 && grad.size(0) <= INT32_MAX,
+                "grad must be a torch.bfloat16 tensor like the rows");
+    check_map(at_row, std::nullopt, grad);
+    const c10::cuda::CUDAGuard guard(grad.device());
+    return combine_run(plain_rows(grad), at_row, std::nullopt);
+}
 // The gradients of combine: of `rows` where n_rows is no less than 0, of the weights where `rows` are there.
 std::tuple<Tensor, Tensor> combine_grads(const Tensor& grad, const std::optional<Tensor>& rows, int64_t n_rows, const Tensor& at_row,
                                          const std::optional<Tensor>& w) {
     const int64_t h = grad.size(-1), k = at_row.size(-1), tokens = at_row.numel() / k;
     const bool need_rows = n_rows >= 0, need_weights = rows.has_value();
-    Tensor d = grad.contiguous();
-    if (reinterpret_cast<uintptr_t>(d.const_data_ptr()) % 16 != 0) d = d.clone();
+    const Tensor d = plain_rows(grad);
     Tensor d_rows = new_cuda({need_rows ? n_rows : 0, h}, at::kBFloat16, grad);
     Tensor d_w = need_weights ? new_cuda(at_row.sizes(), at::kFloat, grad) : new_cuda({0}, at::kFloat, grad);
     if (!need_rows && !need_weights) return {d_rows, d_w};
@@ -406,14 +421,41 @@ Tensor call_combine_rows_grad(const Tensor& g, const Tensor& at_row, const std::
     static const auto h = op<Tensor(const Tensor&, const Tensor&, const std::optional<Tensor>&, c10::SymInt)>("torch_ggml_ops_b200::moe_combine_rows_grad");
     return h.call(g, at_row, w, std::move(n_rows));
 }
+Tensor call_dispatch_grad(const Tensor& g, const Tensor& at_row) {
+    static const auto h = op<Tensor(const Tensor&, const Tensor&)>("torch_ggml_ops_b200::moe_dispatch_grad");
+    return h.call(g, at_row);
+}
 struct DispatchFormula : public Formula {
     using Formula::Formula;
     void gradients(const Tensor& g, variable_list& d) override {
-        // contiguous rows of a multiple of 8 elements start at 16 bytes in whatever tensor they are a part of
-        if (task_should_compute_output(0)) d[0] = call_combine(g.contiguous(), kept[0].unpack(), std::nullopt);
+        if (task_should_compute_output(0)) d[0] = call_dispatch_grad(g, kept[0].unpack());
     }
     std::string name() const override { return "MoeDispatchBackward"; }
 };
+// dispatch is linear, its gradient, too
+struct DispatchGradFormula : public Formula {
+    using Formula::Formula;
+    void gradients(const Tensor& g, variable_list& d) override {
+        if (task_should_compute_output(0)) d[0] = call_combine_rows_grad(g, kept[0].unpack(), std::nullopt, rows);
+    }
+    std::string name() const override { return "MoeDispatchGradBackward"; }
+};
+Tensor dispatch_grad_autograd(const Tensor& g, const Tensor& at_row) {
+    if (!wants_grad(g)) {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        return call_dispatch_grad(g, at_row);
+    }
+    const auto node = formula<DispatchGradFormula>({g});
+    Tensor d;
+    {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        d = call_dispatch_grad(g, at_row);
+    }
+    torch::autograd::set_history(d, node);
+    node->keep({at_row});
+    node->rows = g.sym_size(0);
+    return d;
+}
 std::tuple<Tensor, Tensor, Tensor, Tensor> dispatch_autograd(const Tensor& x, const Tensor& ids, int64_t experts) {
     if (!wants_grad(x)) {
         at::AutoDispatchBelowADInplaceOrView guard;
@@ -643,6 +685,7 @@ TORCH_LIBRARY_FRAGMENT(torch_ggml_ops_b200, m) {
     m.def("moe_balance_loss(Tensor logits, Tensor expert_ids, int scoring) -> (Tensor, Tensor, Tensor)");
     m.def("moe_balance_grad(Tensor grad, Tensor logits, Tensor expert_ids, Tensor coef, int scoring) -> Tensor");
     m.def("moe_dispatch(Tensor input, Tensor expert_ids, int num_experts) -> (Tensor, Tensor, Tensor, Tensor)");
+    m.def("moe_dispatch_grad(Tensor grad, Tensor row_of_pair) -> Tensor");
     m.def("moe_combine(Tensor rows, Tensor row_of_pair, Tensor? weights) -> Tensor");
     m.def("moe_combine_grad(Tensor grad, Tensor rows, Tensor row_of_pair, Tensor? weights, bool need_rows, bool need_weights) -> (Tensor, Tensor)");
     m.def("moe_combine_rows_grad(Tensor grad, Tensor row_of_pair, Tensor? weights, SymInt n_rows) -> Tensor");
@@ -659,6 +702,7 @@ TORCH_LIBRARY_IMPL(torch_ggml_ops_b200, CUDA, m) {
     m.impl("moe_balance_loss", &balance_cuda);
     m.impl("moe_balance_grad", &balance_grad_cuda);
     m.impl("moe_dispatch", &dispatch_cuda);
+    m.impl("moe_dispatch_grad", &dispatch_grad_cuda);
     m.impl("moe_combine", &combine_cuda);
     m.impl("moe_combine_grad", &combine_grad_cuda);
     m.impl("moe_combine_rows_grad", &combine_rows_grad_cuda);
@@ -671,6 +715,7 @@ TORCH_LIBRARY_IMPL(torch_ggml_ops_b200, Autograd, m) {
     m.impl("moe_balance_loss", &balance_autograd);
     m.impl("moe_balance_grad", &balance_grad_autograd);
     m.impl("moe_dispatch", &dispatch_autograd);
+    m.impl("moe_dispatch_grad", &dispatch_grad_autograd);
     m.impl("moe_combine", &combine_autograd);
     m.impl("moe_combine_grad", &combine_grad_autograd);
     m.impl("moe_combine_rows_grad", &combine_rows_grad_autograd);

@@ -51,6 +51,11 @@ def _(input, expert_ids, num_experts):
             expert_ids.new_empty((num_experts,), dtype=torch.int64), expert_ids.new_empty((num_experts,)))
 
 
+@torch.library.register_fake(f"{_NS}::moe_dispatch_grad")
+def _(grad, row_of_pair):
+    return grad.new_empty((*row_of_pair.shape[:-1], grad.shape[1]))
+
+
 @torch.library.register_fake(f"{_NS}::moe_combine")
 def _(rows, row_of_pair, weights):
     return rows.new_empty((*row_of_pair.shape[:-1], rows.shape[1]))
