@@ -105,8 +105,8 @@ __global__ void __launch_bounds__(kMoveThreads) pair_count_kernel(const int32_t*
     __shared__ int32_t hist[kSortExperts];
     for (int e = threadIdx.x; e < experts; e += kMoveThreads) hist[e] = 0;
     __syncthreads();
-    const int i = blockIdx.x * kSortPairs + threadIdx.x;
-    const int e = i < pairs ? ids[i] : -1;
+    const unsigned i = blockIdx.x * kSortPairs + threadIdx.x;   // up to 2^31 + 254
+    const int e = i < static_cast<unsigned>(pairs) ? ids[i] : -1;
     if (e >= 0 && e < experts) atomicAdd(&hist[e], 1);
     __syncthreads();
     for (int k = threadIdx.x; k < experts; k += kMoveThreads) counts[static_cast<size_t>(blockIdx.x) * experts + k] = hist[k];
@@ -177,8 +177,9 @@ __global__ void __launch_bounds__(kMoveThreads) pair_rows_kernel(const int32_t* 
         }
         __syncthreads();
     }
-    const int i = blockIdx.x * kSortPairs + threadIdx.x;
-    int e = i < pairs ? ids[i] : -1;
+    const unsigned i = blockIdx.x * kSortPairs + threadIdx.x;   // up to 2^31 + 254
+    const bool in = i < static_cast<unsigned>(pairs);
+    int e = in ? ids[i] : -1;
     if (e >= experts) e = -1;
     const unsigned same = __match_any_sync(0xFFFFFFFFu, e);
     const int rank = __popc(same & ((1u << lane) - 1u));
@@ -187,7 +188,7 @@ __global__ void __launch_bounds__(kMoveThreads) pair_rows_kernel(const int32_t* 
     int before = rank;
     if (e >= 0)
         for (int w = 0; w < warp; ++w) before += seen[w][e];
-    if (i < pairs) row_of_pair[i] = e >= 0 ? first[e] + before : -1;
+    if (in) row_of_pair[i] = e >= 0 ? first[e] + before : -1;
 }
 
 // A token's row to the rows of its pairs; zeros to the rows behind the last expert's (those of the pairs that name no expert).

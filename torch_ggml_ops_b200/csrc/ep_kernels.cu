@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(256) ep_map_kernel(const int32_t* __restrict__
                                                      const int32_t* __restrict__ dst_base, const int32_t* __restrict__ seg_start,
                                                      int n_pairs, int E, int EL, int capacity, int32_t* __restrict__ dst_rank,
                                                      int32_t* __restrict__ dst_row, int* __restrict__ overflow) {
-    const int i = blockIdx.x * 256 + threadIdx.x;
+    const long long i = blockIdx.x * 256LL + threadIdx.x;
     if (i >= n_pairs) return;
     const int e = expert_ids[i];
     const int j = pair_to_sorted[i];

@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(256) local_plan_kernel(const int32_t* __restri
                                                          const float* __restrict__ pair_weights, int n, int num_experts, int capacity,
                                                          int32_t* __restrict__ pair_row, int32_t* __restrict__ ends,
                                                          float* __restrict__ row_weight, int32_t* __restrict__ overflow) {
-    const int i = blockIdx.x * 256 + threadIdx.x;
+    const long long i = blockIdx.x * 256LL + threadIdx.x;
     if (i == 0) *overflow = expert_ends[num_experts - 1] > capacity ? 1 : 0;
     if (i < num_experts) ends[i] = min(expert_ends[i], capacity);
     if (i >= n) return;
@@ -324,7 +324,7 @@ int tgo_route_sort(const int32_t* expert_ids, int64_t n_pairs, int64_t num_exper
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int n = static_cast<int>(n_pairs), E = static_cast<int>(num_experts);
     const int rounds = route_rounds(n_pairs);
-    const int blocks = (n + kRouteBlock * rounds - 1) / (kRouteBlock * rounds);
+    const int blocks = static_cast<int>((n_pairs + kRouteBlock * rounds - 1) / (kRouteBlock * rounds));
     int32_t* counts = static_cast<int32_t*>(workspace);
     route_count_kernel<<<blocks, kRouteBlock, E * sizeof(int32_t), s>>>(expert_ids, n, E, rounds, counts);
     route_scan_kernel<<<1, 1024, 0, s>>>(counts, blocks, E, expert_indices, expert_offsets, expert_counts);
