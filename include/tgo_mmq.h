@@ -400,8 +400,9 @@ int tgo_moe_dispatch(const void* x, const int32_t* expert_ids, int64_t tokens, i
 int tgo_moe_combine(const void* rows, int64_t n_rows, const int32_t* row_of_pair, const float* weights, void* out, int64_t tokens,
                     int64_t top_k, int64_t width, void* stream);
 /* Its gradients: d_rows [n_rows][width] (null: not wanted; zeros where no pair names the row, the sum where several
- * do) and d_weights fp32 [tokens][top_k] (null: not wanted; 0 for pairs without a row; needs rows).  workspace:
- * n_rows * 4 bytes if d_rows is wanted. */
+ * do, added in their order) and d_weights fp32 [tokens][top_k] (null: not wanted; 0 for pairs without a row; needs rows).
+ * workspace: wanted for d_rows alone; linear in rows and pairs, as the time is, whatever the map. */
+int64_t tgo_moe_combine_grad_workspace_bytes(int64_t n_pairs, int64_t n_rows);
 int tgo_moe_combine_grad(const void* dy, const void* rows, int64_t n_rows, const int32_t* row_of_pair, const float* weights,
                          void* d_rows, float* d_weights, int64_t tokens, int64_t top_k, int64_t width, void* workspace,
                          int64_t workspace_bytes, void* stream);

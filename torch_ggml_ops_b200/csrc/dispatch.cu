@@ -242,23 +242,117 @@ __global__ void __launch_bounds__(kMoveThreads) moe_combine_kernel(const uint4* 
     }
 }
 
-// how many pairs name each row
-__global__ void __launch_bounds__(kMoveThreads) count_rows_kernel(const int32_t* __restrict__ row_of_pair, long long pairs, long long n_rows,
-                                                                  int32_t* __restrict__ count) {
-    const long long i = blockIdx.x * static_cast<long long>(kMoveThreads) + threadIdx.x;
-    if (i >= pairs) return;
-    const int row = row_of_pair[i];
-    if (row >= 0 && row < n_rows) atomicAdd(&count[row], 1);
+// How many pairs name each row.  A map that dispatch makes names a row once at most.  Where one is named more often, the last block to be done
+// lists the pairs of such rows, sorted by row and, of a row, in their order (a radix sort by one block, 8 bits a pass: linear in the pairs, and
+// the maps that are the rule pay no launch for it, but 0.4 to 1.7 us).  Such a row's count becomes -1 - its first place in the list.
+// Gradients of rows and weights, rows of 2048, every row named by two pairs / all pairs naming one row: 65536 pairs 0.6 / 14 ms, 524288 6 / 141 ms.
+constexpr int kListThreads = 1024, kListWarps = kListThreads / 32;
+struct RowLists {
+    int32_t* count;        // [n_rows]
+    int32_t* state;        // blocks that are done; whether a row is named twice; the list's length
+    int32_t *even, *odd;   // [pairs] each: where passes 0, 2 and 1, 3 leave the list
+    int passes;            // bytes of a row's number
+    __device__ int32_t* after(int pass) const { return pass & 1 ? odd : even; }
+};
+__global__ void __launch_bounds__(kListThreads) count_rows_kernel(const int32_t* __restrict__ row_of_pair, long long pairs, long long n_rows, RowLists l) {
+    const long long i = blockIdx.x * static_cast<long long>(kListThreads) + threadIdx.x;
+    bool again = false;
+    if (i < pairs) {
+        const int row = row_of_pair[i];
+        if (row >= 0 && row < n_rows) again = atomicAdd(&l.count[row], 1) != 0;
+    }
+    again = __syncthreads_or(again);
+    __shared__ bool last;
+    if (threadIdx.x == 0) {
+        if (again) atomicOr(&l.state[1], 1);
+        __threadfence();                          // the whole block's counts, which the barrier has put in front of it
+        last = atomicAdd(&l.state[0], 1) == static_cast<int32_t>(gridDim.x) - 1;
+    }
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    if (__ldcg(&l.state[1]) == 0) return;
+
+    __shared__ int32_t next[256];                 // where a digit's next entry goes
+    __shared__ uint16_t seen[kListWarps][256];    // a step's entries of a digit per warp, then in the warps in front
+    __shared__ int32_t total;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long n = pairs;                          // the first pass looks at all pairs and takes those of rows that are named again
+    for (int pass = 0; pass < l.passes; ++pass) {
+        const int32_t* from = l.after(pass - 1);
+        int32_t* to = l.after(pass);
+        int digit;                                // of the entry that was looked at last; -1: none
+        auto entry = [&](long long k) {
+            digit = -1;
+            if (k >= n) return -1;
+            const int p = pass == 0 ? static_cast<int>(k) : __ldcg(from + k);
+            const int row = row_of_pair[p];
+            if (pass > 0 || (row >= 0 && row < n_rows && __ldcg(&l.count[row]) > 1)) digit = row >> (8 * pass) & 255;
+            return p;
+        };
+        if (threadIdx.x < 256) next[threadIdx.x] = 0;
+        __syncthreads();
+        for (long long k = threadIdx.x; k < n; k += kListThreads) {
+            entry(k);
+            if (digit >= 0) atomicAdd(&next[digit], 1);
+        }
+        __syncthreads();
+        if (warp == 0) {
+            int carry = 0;
+            for (int d0 = 0; d0 < 256; d0 += 32) {
+                const int own = next[d0 + lane];
+                int upto = own;
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const int o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+                    if (lane >= d) upto += o;
+                }
+                next[d0 + lane] = carry + upto - own;
+                carry += __shfl_sync(0xFFFFFFFFu, upto, 31);
+            }
+            if (lane == 0) total = carry;
+        }
+        for (long long k0 = 0; k0 < n; k0 += kListThreads) {
+            for (int k = threadIdx.x; k < kListWarps * 256; k += kListThreads) (&seen[0][0])[k] = 0;
+            const int p = entry(k0 + threadIdx.x);
+            __syncthreads();
+            const unsigned same = __match_any_sync(0xFFFFFFFFu, digit);
+            const int rank = __popc(same & ((1u << lane) - 1u));
+            if (digit >= 0 && rank == 0) seen[warp][digit] = static_cast<uint16_t>(__popc(same));
+            __syncthreads();
+            int here = 0;
+            if (threadIdx.x < 256) {
+                for (int w = 0; w < kListWarps; ++w) {
+                    const int c = seen[w][threadIdx.x];
+                    seen[w][threadIdx.x] = static_cast<uint16_t>(here);
+                    here += c;
+                }
+            }
+            __syncthreads();
+            if (digit >= 0) to[next[digit] + seen[warp][digit] + rank] = p;
+            __syncthreads();
+            if (threadIdx.x < 256) next[threadIdx.x] += here;
+        }
+        __syncthreads();
+        n = total;
+    }
+    const int32_t* sorted = l.after(l.passes - 1);
+    for (long long k = threadIdx.x; k < n; k += kListThreads) {
+        const int row = row_of_pair[__ldcg(sorted + k)];
+        if (k == 0 || row_of_pair[__ldcg(sorted + k - 1)] != row) l.count[row] = static_cast<int32_t>(-1 - k);
+    }
+    if (threadIdx.x == 0) l.state[2] = static_cast<int32_t>(n);
 }
 
-// One warp per pair.  A row that several pairs name (dispatch gives none such) gets the sum over them from
-// the first of them, a row that none names zeros from the warp of that number.
+// One warp per pair.  A row that none names gets zeros from the warp of that number, one that several pairs name the sum over them: its
+// columns are divided among the warps of the first 32 of them.
 __global__ void __launch_bounds__(kMoveThreads) combine_grad_kernel(const uint4* __restrict__ dy, const uint4* __restrict__ rows, long long n_rows,
                                                                     const int32_t* __restrict__ row_of_pair, const float* __restrict__ weights,
-                                                                    const int32_t* __restrict__ count, uint4* __restrict__ d_rows,
-                                                                    float* __restrict__ d_weights, long long pairs, int top_k, int vec_per_row) {
+                                                                    RowLists l, uint4* __restrict__ d_rows, float* __restrict__ d_weights,
+                                                                    long long pairs, int top_k, int vec_per_row) {
     const int lane = threadIdx.x & 31;
     const long long pair = blockIdx.x * static_cast<long long>(kMoveThreads / 32) + (threadIdx.x >> 5);
+    const int32_t* count = l.count;
     if (d_rows != nullptr && pair < n_rows && count[pair] == 0)
         for (int c = lane; c < vec_per_row; c += 32) d_rows[pair * vec_per_row + c] = make_uint4(0, 0, 0, 0);
     if (pair >= pairs) return;
@@ -300,19 +394,36 @@ __global__ void __launch_bounds__(kMoveThreads) combine_grad_kernel(const uint4*
             }
         }
         if (!alone) {
-            long long before = 0;
-            while (before < pair && row_of_pair[before] != row) ++before;
-            for (int c = lane; before == pair && c < vec_per_row; c += 32) {
+            const int32_t* list = l.after(l.passes - 1);
+            const long long first = -1 - static_cast<long long>(count[row]), n = l.state[2];
+            // entry k of the list, if it is one of this row; -1 else
+            auto of_row = [&](long long k) {
+                const int p = k < n ? list[k] : -1;
+                return p >= 0 && row_of_pair[p] == row ? p : -1;
+            };
+            const int p0 = of_row(first + lane);
+            const int helpers = __popc(__ballot_sync(0xFFFFFFFFu, p0 >= 0));
+            const unsigned me = __ballot_sync(0xFFFFFFFFu, p0 == pair);
+            for (int c0 = me == 0 ? vec_per_row : 32 * (__ffs(me) - 1); c0 < vec_per_row; c0 += 32 * helpers) {
+                const int c = c0 + lane;
                 float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                for (long long p = pair; p < pairs; ++p) {
-                    if (row_of_pair[p] != row) continue;
-                    const float wp = weights != nullptr ? weights[p] : 1.0f;
-                    float f[8];
-                    widen(dy[p / top_k * vec_per_row + c], f);
+                int m = 32;
+                for (long long k = first; m == 32; k += 32) {
+                    const int p = of_row(k + lane);
+                    const float wp = p >= 0 && weights != nullptr ? weights[p] : 1.0f;
+                    m = __popc(__ballot_sync(0xFFFFFFFFu, p >= 0));
+#pragma unroll 4
+                    for (int j = 0; j < m; ++j) {
+                        const int q = __shfl_sync(0xFFFFFFFFu, p, j);
+                        const float w = __shfl_sync(0xFFFFFFFFu, wp, j);
+                        if (c >= vec_per_row) continue;
+                        float f[8];
+                        widen(dy[static_cast<long long>(q / top_k) * vec_per_row + c], f);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) acc[j] = fmaf(wp, f[j], acc[j]);
+                        for (int u = 0; u < 8; ++u) acc[u] = fmaf(w, f[u], acc[u]);
+                    }
                 }
-                d_rows[static_cast<long long>(row) * vec_per_row + c] = narrow(acc);
+                if (c < vec_per_row) d_rows[static_cast<long long>(row) * vec_per_row + c] = narrow(acc);
             }
         }
     }
@@ -406,6 +517,11 @@ int tgo_moe_combine(const void* rows, int64_t n_rows, const int32_t* row_of_pair
     return launched("moe_combine_kernel launch failed");
 }
 
+int64_t tgo_moe_combine_grad_workspace_bytes(int64_t n_pairs, int64_t n_rows) {
+    if (n_pairs < 0 || n_rows < 0) return -1;
+    return (n_rows + 3 + 2 * n_pairs) * 4;
+}
+
 int tgo_moe_combine_grad(const void* dy, const void* rows, int64_t n_rows, const int32_t* row_of_pair, const float* weights, void* d_rows,
                          float* d_weights, int64_t tokens, int64_t top_k, int64_t width, void* workspace, int64_t workspace_bytes, void* stream) {
     if (dy == nullptr || row_of_pair == nullptr || (d_weights != nullptr && rows == nullptr)) return route_fail(TGO_E_ARG, "null pointer");
@@ -416,17 +532,23 @@ int tgo_moe_combine_grad(const void* dy, const void* rows, int64_t n_rows, const
     if (!a16(dy) || !a16(rows) || !a16(d_rows)) return route_fail(TGO_E_ARG, "data pointers must be 16-byte aligned");
     const int64_t pairs = tokens * top_k;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    int32_t* count = static_cast<int32_t*>(workspace);
+    RowLists l = {};
     int64_t items = pairs;
     if (d_rows != nullptr) {
         if (reinterpret_cast<uintptr_t>(workspace) % 4 != 0) return route_fail(TGO_E_ARG, "the workspace must be 4-byte aligned");
-        if (workspace == nullptr || workspace_bytes < n_rows * 4) return route_fail(TGO_E_WORKSPACE, "combine workspace is smaller than n_rows * 4 bytes");
-        if (cudaMemsetAsync(count, 0, static_cast<size_t>(n_rows) * 4, st) != cudaSuccess) return route_fail(TGO_E_CUDA, "cudaMemsetAsync failed");
-        count_rows_kernel<<<static_cast<unsigned>((pairs + kMoveThreads - 1) / kMoveThreads), kMoveThreads, 0, st>>>(row_of_pair, pairs, n_rows, count);
+        if (workspace == nullptr || workspace_bytes < tgo_moe_combine_grad_workspace_bytes(pairs, n_rows))
+            return route_fail(TGO_E_WORKSPACE, "combine workspace too small");
+        l.count = static_cast<int32_t*>(workspace);
+        l.state = l.count + n_rows;
+        l.even = l.state + 3;
+        l.odd = l.even + pairs;
+        for (l.passes = 1; l.passes < 4 && (n_rows - 1) >> (8 * l.passes) > 0;) ++l.passes;
+        if (cudaMemsetAsync(l.count, 0, static_cast<size_t>(n_rows + 3) * 4, st) != cudaSuccess) return route_fail(TGO_E_CUDA, "cudaMemsetAsync failed");
+        count_rows_kernel<<<static_cast<unsigned>((pairs + kListThreads - 1) / kListThreads), kListThreads, 0, st>>>(row_of_pair, pairs, n_rows, l);
         if (n_rows > items) items = n_rows;
     }
     combine_grad_kernel<<<static_cast<unsigned>((items + kMoveThreads / 32 - 1) / (kMoveThreads / 32)), kMoveThreads, 0, st>>>(
-        static_cast<const uint4*>(dy), static_cast<const uint4*>(rows), n_rows, row_of_pair, weights, count, static_cast<uint4*>(d_rows), d_weights,
+        static_cast<const uint4*>(dy), static_cast<const uint4*>(rows), n_rows, row_of_pair, weights, l, static_cast<uint4*>(d_rows), d_weights,
         pairs, static_cast<int>(top_k), static_cast<int>(width / 8));
     return launched("combine gradient kernel launch failed");
 }

@@ -371,7 +371,7 @@ std::tuple<Tensor, Tensor> combine_grads(const Tensor& grad, const std::optional
     if (!need_rows && !need_weights) return {d_rows, d_w};
     const int64_t existing = need_weights ? rows->size(0) : n_rows;
     if (existing == 0 || tokens == 0) return {d_rows.zero_(), d_w.zero_()};
-    const int64_t bytes = need_rows ? n_rows * 4 : 0;
+    const int64_t bytes = need_rows ? tgo_moe_combine_grad_workspace_bytes(at_row.numel(), n_rows) : 0;
     const Tensor ws = bytes > 0 ? new_cuda({bytes}, at::kByte, grad) : Tensor();
     check_rc(tgo_moe_combine_grad(d.const_data_ptr(), need_weights ? rows->const_data_ptr() : nullptr, existing, at_row.const_data_ptr<int32_t>(),
                                   w.has_value() ? w->const_data_ptr<float>() : nullptr, need_rows ? d_rows.mutable_data_ptr() : nullptr,

@@ -39,6 +39,7 @@ SIGNATURES = {
     "tgo_moe_dispatch_workspace_bytes": (_i64, [_i64, _i64]),
     "tgo_moe_dispatch": (_i32, [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
     "tgo_moe_combine": (_i32, [_vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
+    "tgo_moe_combine_grad_workspace_bytes": (_i64, [_i64, _i64]),
     "tgo_moe_combine_grad": (_i32, [_vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp]),
     "tgo_logit_rules": (_i32, [_vp, _vp, _i32, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i32, _i32, _vp, ctypes.c_float, _vp,
                                ctypes.c_float, _vp, ctypes.c_float, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _i64, _vp]),
