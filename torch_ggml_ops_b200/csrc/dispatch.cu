@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(kScanWarps * 32) pair_scan_kernel(int32_t* __r
 __global__ void __launch_bounds__(kMoveThreads) pair_rows_kernel(const int32_t* __restrict__ ids, int pairs, int experts, const int32_t* __restrict__ starts,
                                                                  const int32_t* __restrict__ totals, int32_t* __restrict__ row_of_pair,
                                                                  int64_t* __restrict__ expert_indices, int32_t* __restrict__ expert_offsets) {
-    __shared__ uint16_t seen[kMoveWarps][kSortExperts];   // pairs of an expert per warp, then in the warps in front
+    __shared__ __align__(16) uint16_t seen[kMoveWarps][kSortExperts];   // pairs of an expert per warp, then in the warps in front
     __shared__ int32_t first[kSortExperts];               // an expert's first row of this block
     __shared__ int32_t warp_sum[kMoveWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
