@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(kListThreads) count_rows_kernel(const int32_t*
     if (__ldcg(&l.state[1]) == 0) return;
 
     __shared__ int32_t next[256];                 // where a digit's next entry goes
-    __shared__ uint16_t seen[kListWarps][256];    // a step's entries of a digit per warp, then in the warps in front
+    __shared__ uint16_t among[kListWarps][256];    // a step's entries of a digit per warp, then in the warps in front
     __shared__ int32_t total;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     long long n = pairs;                          // the first pass looks at all pairs and takes those of rows that are named again
@@ -313,23 +313,23 @@ __global__ void __launch_bounds__(kListThreads) count_rows_kernel(const int32_t*
             if (lane == 0) total = carry;
         }
         for (long long k0 = 0; k0 < n; k0 += kListThreads) {
-            for (int k = threadIdx.x; k < kListWarps * 256; k += kListThreads) (&seen[0][0])[k] = 0;
+            for (int k = threadIdx.x; k < kListWarps * 256; k += kListThreads) (&among[0][0])[k] = 0;
             const int p = entry(k0 + threadIdx.x);
             __syncthreads();
             const unsigned same = __match_any_sync(0xFFFFFFFFu, digit);
             const int rank = __popc(same & ((1u << lane) - 1u));
-            if (digit >= 0 && rank == 0) seen[warp][digit] = static_cast<uint16_t>(__popc(same));
+            if (digit >= 0 && rank == 0) among[warp][digit] = static_cast<uint16_t>(__popc(same));
             __syncthreads();
             int here = 0;
             if (threadIdx.x < 256) {
                 for (int w = 0; w < kListWarps; ++w) {
-                    const int c = seen[w][threadIdx.x];
-                    seen[w][threadIdx.x] = static_cast<uint16_t>(here);
+                    const int c = among[w][threadIdx.x];
+                    among[w][threadIdx.x] = static_cast<uint16_t>(here);
                     here += c;
                 }
             }
             __syncthreads();
-            if (digit >= 0) to[next[digit] + seen[warp][digit] + rank] = p;
+            if (digit >= 0) to[next[digit] + among[warp][digit] + rank] = p;
             __syncthreads();
             if (threadIdx.x < 256) next[threadIdx.x] += here;
         }
