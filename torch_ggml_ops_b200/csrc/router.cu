@@ -595,18 +595,21 @@ static int check_scores(const void* logits, int dtype, int64_t tokens, int64_t e
 }
 static int launched(const char* what) { return cudaGetLastError() == cudaSuccess ? TGO_OK : route_fail(TGO_E_CUDA, what); }
 static unsigned token_blocks(int64_t tokens) { return static_cast<unsigned>((tokens + kRouterWarps - 1) / kRouterWarps); }
-// for kernels whose warps take one token after another: as many blocks as run at once
-template <auto KERNEL>
-static unsigned resident_blocks(int64_t tokens, size_t smem = 0) {
+// for kernels whose warps take one token after another: as many blocks as run at once.  SMEM: the most shared memory that the kernel is ever
+// given, so that a grid, and with it the order of a sum, depends on the call alone and not on the calls before it.
+template <auto KERNEL, size_t SMEM = 0>
+static unsigned resident_blocks(int64_t tokens) {
     static std::atomic<int> per_sm{0};
     int n = per_sm.load(std::memory_order_relaxed);
     if (n == 0) {
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, KERNEL, kRouterWarps * 32, smem) != cudaSuccess || n < 1) n = 1;
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, KERNEL, kRouterWarps * 32, SMEM) != cudaSuccess || n < 1) n = 1;
         per_sm.store(n, std::memory_order_relaxed);
     }
     const unsigned b = token_blocks(tokens);
     return b < 148u * n ? b : 148u * n;
 }
+// balance_kernel's: pairs of every expert, the tokens, the warps' sums
+static constexpr size_t balance_smem(int64_t experts) { return ((kRouterWarps + 1) * experts + 1) * 4; }
 
 // log2(tokens), rounded up
 static int bits_of(int64_t tokens) {
@@ -677,14 +680,14 @@ int tgo_moe_balance_loss(const void* logits, int dtype, int64_t tokens, int64_t 
     const BalanceSums sums = {static_cast<unsigned long long*>(workspace), reinterpret_cast<int32_t*>(static_cast<unsigned long long*>(workspace) + experts),
                               62 - bits_of(tokens)};
     if (cudaMemsetAsync(workspace, 0, static_cast<size_t>(experts) * 12 + 12, st) != cudaSuccess) return route_fail(TGO_E_CUDA, "cudaMemsetAsync failed");
-    const size_t smem = ((kRouterWarps + 1) * experts + 1) * 4;
+    const size_t smem = balance_smem(experts);
     return with_layout(dtype, experts, [&](auto t, auto vpl) {
         using T = decltype(t);
         constexpr int VPL = decltype(vpl)::value;
         const BalanceArgs a = {logits, tokens, row_stride, static_cast<int>(experts), static_cast<int>(top_k),
                                RowLayout<T, VPL>::whole_chunks(logits, experts, row_stride), expert_ids};
-        if (scoring == TGO_SCORING_SIGMOID) balance_kernel<T, VPL, true><<<resident_blocks<balance_kernel<T, VPL, true>>(tokens, smem), kRouterWarps * 32, smem, st>>>(a, sums, loss, counts, coef);
-        else balance_kernel<T, VPL, false><<<resident_blocks<balance_kernel<T, VPL, false>>(tokens, smem), kRouterWarps * 32, smem, st>>>(a, sums, loss, counts, coef);
+        if (scoring == TGO_SCORING_SIGMOID) balance_kernel<T, VPL, true><<<resident_blocks<balance_kernel<T, VPL, true>, balance_smem(32 * VPL)>(tokens), kRouterWarps * 32, smem, st>>>(a, sums, loss, counts, coef);
+        else balance_kernel<T, VPL, false><<<resident_blocks<balance_kernel<T, VPL, false>, balance_smem(32 * VPL)>(tokens), kRouterWarps * 32, smem, st>>>(a, sums, loss, counts, coef);
         return launched("balance_kernel launch failed");
     });
 }
