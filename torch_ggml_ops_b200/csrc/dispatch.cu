@@ -15,6 +15,8 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include "aligned.h"
+
 namespace tgo {
 
 int route_fail(int code, const char* msg);  // tgo_api.cu
@@ -434,7 +436,6 @@ __global__ void __launch_bounds__(kMoveThreads) combine_grad_kernel(const uint4*
     }
 }
 
-static bool a16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 static int launched(const char* what) { return cudaGetLastError() == cudaSuccess ? TGO_OK : route_fail(TGO_E_CUDA, what); }
 static int check_rows(int64_t tokens, int64_t top_k, int64_t width) {
     if (tokens <= 0) return route_fail(TGO_E_ARG, "zero-row inputs are not supported");
@@ -470,12 +471,13 @@ int tgo_moe_dispatch(const void* x, const int32_t* expert_ids, int64_t tokens, i
         return route_fail(TGO_E_ARG, "null pointer");
     int rc = check_rows(tokens, top_k, width);
     if (rc != TGO_OK) return rc;
-    if (!a16(x) || !a16(rows)) return route_fail(TGO_E_ARG, "data pointers must be 16-byte aligned");
+    if (!aligned_to(16, x, rows)) return route_fail(TGO_E_ARG, "data pointers must be 16-byte aligned");
+    if (!aligned_to(4, expert_ids, row_of_pair, expert_offsets) || !aligned_to(8, expert_indices)) return route_fail(TGO_E_ARG, kMisaligned);
     const int64_t pairs = tokens * top_k;
     if (num_experts <= 0 || num_experts > 4096) return route_fail(TGO_E_ARG, "num_experts must be in 1..4096");
     const int64_t need = tgo_moe_dispatch_workspace_bytes(pairs, num_experts);
     if (workspace_bytes < need || (need > 0 && workspace == nullptr)) return route_fail(TGO_E_WORKSPACE, "dispatch workspace too small");
-    if (reinterpret_cast<uintptr_t>(workspace) % 4 != 0) return route_fail(TGO_E_ARG, "the workspace must be 4-byte aligned");
+    if (!aligned_to(4, workspace)) return route_fail(TGO_E_ARG, "the workspace must be 4-byte aligned");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int vec = static_cast<int>(width / 8), n = static_cast<int>(pairs), e = static_cast<int>(num_experts);
     if (need == 0) {
@@ -510,7 +512,8 @@ int tgo_moe_combine(const void* rows, int64_t n_rows, const int32_t* row_of_pair
     const int rc = check_rows(tokens, top_k, width);
     if (rc != TGO_OK) return rc;
     if (n_rows < 0) return route_fail(TGO_E_ARG, "a negative number of rows");
-    if (!a16(rows) || !a16(out)) return route_fail(TGO_E_ARG, "data pointers must be 16-byte aligned");
+    if (!aligned_to(16, rows, out)) return route_fail(TGO_E_ARG, "data pointers must be 16-byte aligned");
+    if (!aligned_to(4, row_of_pair, weights)) return route_fail(TGO_E_ARG, kMisaligned);
     const int vec = static_cast<int>(width / 8);
     moe_combine_kernel<<<move_grid(tokens * vec), kMoveThreads, 0, static_cast<cudaStream_t>(stream)>>>(
         static_cast<const uint4*>(rows), n_rows, row_of_pair, weights, static_cast<uint4*>(out), tokens, static_cast<int>(top_k), vec);
@@ -529,13 +532,14 @@ int tgo_moe_combine_grad(const void* dy, const void* rows, int64_t n_rows, const
     const int rc = check_rows(tokens, top_k, width);
     if (rc != TGO_OK) return rc;
     if (n_rows < 0 || n_rows > INT32_MAX) return route_fail(TGO_E_ARG, "the number of rows must be in 0..2^31-1");
-    if (!a16(dy) || !a16(rows) || !a16(d_rows)) return route_fail(TGO_E_ARG, "data pointers must be 16-byte aligned");
+    if (!aligned_to(16, dy, rows, d_rows)) return route_fail(TGO_E_ARG, "data pointers must be 16-byte aligned");
+    if (!aligned_to(4, row_of_pair, weights, d_weights)) return route_fail(TGO_E_ARG, kMisaligned);
     const int64_t pairs = tokens * top_k;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     RowLists l = {};
     int64_t items = pairs;
     if (d_rows != nullptr) {
-        if (reinterpret_cast<uintptr_t>(workspace) % 4 != 0) return route_fail(TGO_E_ARG, "the workspace must be 4-byte aligned");
+        if (!aligned_to(4, workspace)) return route_fail(TGO_E_ARG, "the workspace must be 4-byte aligned");
         if (workspace == nullptr || workspace_bytes < tgo_moe_combine_grad_workspace_bytes(pairs, n_rows))
             return route_fail(TGO_E_WORKSPACE, "combine workspace too small");
         l.count = static_cast<int32_t*>(workspace);

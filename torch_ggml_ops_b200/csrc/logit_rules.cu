@@ -24,6 +24,7 @@
 
 #include <atomic>
 
+#include "aligned.h"
 #include "scores.cuh"
 
 namespace tgo {
@@ -397,6 +398,9 @@ extern "C" int tgo_logit_rules(const void* logits, void* out, int dtype, int64_t
     const int64_t size = dtype == TGO_FP32 ? 4 : 2;
     const uintptr_t i = reinterpret_cast<uintptr_t>(logits), o = reinterpret_cast<uintptr_t>(out);
     if (i % size != 0 || o % size != 0) return route_fail(TGO_E_ARG, "logits are not aligned to their type");
+    if ((history != nullptr && (!aligned_to(history_id_bytes, history) || (lengths != nullptr && !aligned_to(length_bytes, lengths)))) ||
+        (bias_ids != nullptr && !aligned_to(bias_id_bytes, bias_ids)) || !aligned_to(4, repetition, presence, frequency, bias_values, allowed))
+        return route_fail(TGO_E_ARG, kMisaligned);
     RulesArgs a = {};
     a.logits = logits, a.out = out, a.rows = rows, a.vocab = vocab, a.in_stride = in_stride, a.out_stride = out_stride;
     if (history != nullptr && history_len > 0) a.history = history, a.lengths = lengths, a.history_len = history_len, a.history_stride = history_stride;

@@ -28,6 +28,7 @@
 #include <atomic>
 #include <type_traits>
 
+#include "aligned.h"
 #include "scores.cuh"
 
 namespace tgo {
@@ -589,7 +590,7 @@ static int check_scores(const void* logits, int dtype, int64_t tokens, int64_t e
     if (top_k <= 0 || top_k > kRouterMaxTopK || top_k > experts) return route_fail(TGO_E_ARG, "top_k must be in 1..32 and at most num_experts");
     if (tokens > INT32_MAX / top_k) return route_fail(TGO_E_ARG, "tokens * top_k must be below 2^31");
     if (stride < experts && tokens > 1) return route_fail(TGO_E_ARG, "rows of logits overlap");
-    if (reinterpret_cast<uintptr_t>(logits) % type_bytes(dtype) != 0) return route_fail(TGO_E_ARG, "logits are not aligned to their type");
+    if (!aligned_to(type_bytes(dtype), logits)) return route_fail(TGO_E_ARG, "logits are not aligned to their type");
     if (scoring != TGO_SCORING_SOFTMAX && scoring != TGO_SCORING_SIGMOID) return route_fail(TGO_E_ARG, "unknown scoring");
     return TGO_OK;
 }
@@ -627,6 +628,7 @@ extern "C" {
 int tgo_moe_router(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t row_stride, int64_t top_k, int scoring, int normalize,
                    const uint8_t* token_mask, float* weights, int32_t* expert_ids, void* stream) {
     if (weights == nullptr || expert_ids == nullptr) return route_fail(TGO_E_ARG, "null pointer");
+    if (!aligned_to(4, weights, expert_ids)) return route_fail(TGO_E_ARG, kMisaligned);
     const int rc = check_scores(logits, dtype, tokens, experts, row_stride, top_k, scoring);
     if (rc != TGO_OK) return rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -646,6 +648,7 @@ int tgo_moe_router_grad(const void* logits, int dtype, int64_t tokens, int64_t e
     if (weights == nullptr || expert_ids == nullptr || d_weights == nullptr || d_logits == nullptr) return route_fail(TGO_E_ARG, "null pointer");
     const int rc = check_scores(logits, dtype, tokens, experts, row_stride, top_k, scoring);
     if (rc != TGO_OK) return rc;
+    if (!aligned_to(4, weights, expert_ids, d_weights) || !aligned_to(type_bytes(dtype), d_logits)) return route_fail(TGO_E_ARG, kMisaligned);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return with_layout(dtype, experts, [&](auto t, auto vpl) {
         using T = decltype(t);
@@ -674,6 +677,7 @@ int tgo_moe_balance_loss(const void* logits, int dtype, int64_t tokens, int64_t 
         return route_fail(TGO_E_ARG, "null pointer");
     const int rc = check_scores(logits, dtype, tokens, experts, row_stride, top_k, scoring);
     if (rc != TGO_OK) return rc;
+    if (!aligned_to(4, expert_ids, loss, counts, coef)) return route_fail(TGO_E_ARG, kMisaligned);
     if (workspace_bytes < tgo_moe_balance_workspace_bytes(tokens, experts)) return route_fail(TGO_E_WORKSPACE, "balance workspace too small");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (reinterpret_cast<uintptr_t>(workspace) % 8 != 0) return route_fail(TGO_E_ARG, "the workspace must be 8-byte aligned");
@@ -697,6 +701,7 @@ int tgo_moe_balance_grad(const void* logits, int dtype, int64_t tokens, int64_t 
     if (expert_ids == nullptr || coef == nullptr || d_loss == nullptr || d_logits == nullptr) return route_fail(TGO_E_ARG, "null pointer");
     const int rc = check_scores(logits, dtype, tokens, experts, row_stride, top_k, scoring);
     if (rc != TGO_OK) return rc;
+    if (!aligned_to(4, expert_ids, coef, d_loss) || !aligned_to(type_bytes(dtype), d_logits)) return route_fail(TGO_E_ARG, kMisaligned);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return with_layout(dtype, experts, [&](auto t, auto vpl) {
         using T = decltype(t);
