@@ -412,7 +412,7 @@ int tgo_moe_combine_grad(const void* dy, const void* rows, int64_t n_rows, const
  *   c = occurrences of the token in the first lengths[row] of the row's history_len ids; where c > 0:
  *       x = (x > 0 ? x / repetition : x * repetition) - (c * frequency + presence);
  *   x = -inf where bit (token % 32) of allowed[row][token / 32] is 0;
- * one rounding to `dtype`.  out may be logits itself (with the same strides).  Null: history (nothing is
+ * one rounding to `dtype`.  out may be logits itself (with the same strides) and shares no memory with them else.  Null: history (nothing is
  * penalised), lengths (all history_len ids), allowed (every token), bias_ids (none); repetition, presence,
  * frequency (fp32 [rows]; null: the value beside them).  Ids of 4 or 8 bytes; those outside the vocabulary name
  * nothing.  Strides in elements; a stride of 0 gives every row the same ids or mask. */

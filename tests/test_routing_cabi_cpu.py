@@ -46,3 +46,21 @@ def test_misaligned_pointers_are_refused(name):
     for which, size in pointers.items():
         assert call(**{k: p + (size // 2 if k == which else 0) for k in pointers}) < 0
         assert "align" in native.last_error(), (which, native.last_error())
+
+
+def test_a_result_that_meets_the_logits_is_refused():
+    """out is the logits themselves or shares nothing with them; nothing is left to do for logits that no rule names, so that a legal call needs no
+    device."""
+    from torch_ggml_ops_b200 import native
+
+    lib = native.lib()
+    buf = (ctypes.c_char * 4096)()
+    p = (ctypes.addressof(buf) + 63) & ~63
+
+    def call(out, rows=3, vocab=8, in_stride=20, out_stride=20, allowed=p):
+        return lib.tgo_logit_rules(p, out, 2, rows, vocab, in_stride, out_stride, None, None, 0, 0, 8, 8, None, 1.0, None, 0.0, None, 0.0, None, None, 0, 0, 0, 8, allowed, 1, None)
+
+    for kw in (dict(out=p, out_stride=24), dict(out=p, in_stride=8), dict(out=p + 4), dict(out=p + 28), dict(out=p + 80), dict(out=p + 52), dict(out=p + 4, rows=1),
+               dict(out=p + 28, rows=1), dict(out=p + 100), dict(out=p + 160, out_stride=16)):
+        assert call(**kw) < 0 and "no memory" in native.last_error(), (kw, native.last_error())
+    assert call(out=p, allowed=None) == 0 and call(out=p, rows=1, in_stride=0, out_stride=0, allowed=None) == 0

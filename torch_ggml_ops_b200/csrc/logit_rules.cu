@@ -316,6 +316,17 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logit_rules_kernel(Ru
         [&](int64_t t) { return x[t - s.base + kRulesPad]; });
 }
 
+// Whether two matrices [rows][width] of elements of `size` bytes are the same one or no element of one is in the other: memory that does not
+// meet, or columns of one wider matrix side by side.
+static bool apart_or_same(uintptr_t a, int64_t stride_a, uintptr_t b, int64_t stride_b, int64_t rows, int64_t width, int64_t size) {
+    if (rows == 1) stride_a = stride_b = width;
+    if (a == b && stride_a == stride_b) return true;
+    if (a + ((rows - 1) * stride_a + width) * size <= b || b + ((rows - 1) * stride_b + width) * size <= a) return true;
+    if (stride_a != stride_b) return false;
+    const int64_t d = static_cast<int64_t>((a > b ? a - b : b - a) % (stride_a * size));
+    return d >= width * size && stride_a * size - d >= width * size;
+}
+
 // ------------------------------------------------------------------ launches
 constexpr int64_t kThreadMemory = 220;   // bytes of shared memory per thread: an SM's for 1024
 
@@ -401,6 +412,8 @@ extern "C" int tgo_logit_rules(const void* logits, void* out, int dtype, int64_t
     if ((history != nullptr && (!aligned_to(history_id_bytes, history) || (lengths != nullptr && !aligned_to(length_bytes, lengths)))) ||
         (bias_ids != nullptr && !aligned_to(bias_id_bytes, bias_ids)) || !aligned_to(4, repetition, presence, frequency, bias_values, allowed))
         return route_fail(TGO_E_ARG, kMisaligned);
+    if (!apart_or_same(i, in_stride, o, out_stride, rows, vocab, size))
+        return route_fail(TGO_E_ARG, "out must be the logits themselves or share no memory with them");
     RulesArgs a = {};
     a.logits = logits, a.out = out, a.rows = rows, a.vocab = vocab, a.in_stride = in_stride, a.out_stride = out_stride;
     if (history != nullptr && history_len > 0) a.history = history, a.lengths = lengths, a.history_len = history_len, a.history_stride = history_stride;
@@ -410,7 +423,7 @@ extern "C" int tgo_logit_rules(const void* logits, void* out, int dtype, int64_t
     if (bias_ids != nullptr && n_bias > 0) a.bias_ids = bias_ids, a.bias_values = bias_values, a.n_bias = n_bias;
     a.bias_ids_stride = bias_ids_stride, a.bias_values_stride = bias_values_stride, a.bias_wide = bias_id_bytes == 8;
     a.allowed = allowed, a.allowed_stride = allowed_stride;
-    a.in_place = logits == out && (rows == 1 || in_stride == out_stride);
+    a.in_place = logits == out;
     // 16-byte accesses where every row of the result lies to its boundary as the row of logits does
     a.vectors = (i - o) % 16 == 0 && (rows == 1 || (in_stride - out_stride) * size % 16 == 0);
     cudaStream_t st = static_cast<cudaStream_t>(stream);

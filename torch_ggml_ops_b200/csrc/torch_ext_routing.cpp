@@ -5,7 +5,6 @@
 #include <ATen/MemoryOverlap.h>
 #include <c10/util/ScopeExit.h>
 
-#include <cstdlib>
 #include <mutex>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
@@ -607,19 +606,6 @@ void rules_into(const Tensor& logits, const MaybeTensor& history, const MaybeTen
                              stream_of(logits)),
              "logit_rules");
 }
-// Whether two matrices of one shape are the same one or no element of one is in the other: memory that does not meet, or columns of
-// one wider matrix side by side.
-bool apart_or_same(const Tensor& a, const Tensor& b) {
-    if (a.numel() == 0 || a.sizes() != b.sizes() || a.scalar_type() != b.scalar_type() || a.device() != b.device()) return true;   // refused elsewhere
-    const int64_t width = a.size(-1), rows = a.numel() / width, size = static_cast<int64_t>(a.element_size());
-    const int64_t sa = rows > 1 ? a.stride(0) : width, sb = rows > 1 ? b.stride(0) : width;
-    const intptr_t pa = reinterpret_cast<intptr_t>(a.const_data_ptr()), pb = reinterpret_cast<intptr_t>(b.const_data_ptr());
-    if (pa == pb && sa == sb) return true;
-    if (pa + ((rows - 1) * sa + width) * size <= pb || pb + ((rows - 1) * sb + width) * size <= pa) return true;
-    if (sa != sb || sa <= 0) return false;
-    const int64_t d = std::abs(pa - pb) % (sa * size);
-    return d >= width * size && sa * size - d >= width * size;
-}
 Tensor rules_cuda(const Tensor& logits, const MaybeTensor& history, const MaybeTensor& lengths, const MaybeTensor& repetition, double repetition_all,
                   const MaybeTensor& presence, double presence_all, const MaybeTensor& frequency, double frequency_all, const MaybeTensor& bias_ids,
                   const MaybeTensor& bias_values, const MaybeTensor& allowed) {
@@ -634,7 +620,6 @@ void rules_out_cuda(const Tensor& logits, const MaybeTensor& history, const Mayb
                     const MaybeTensor& presence, double presence_all, const MaybeTensor& frequency, double frequency_all, const MaybeTensor& bias_ids,
                     const MaybeTensor& bias_values, const MaybeTensor& allowed, Tensor& out) {
     at::assert_no_internal_overlap(out);
-    TORCH_CHECK(apart_or_same(logits, out), "out must be logits themselves or share no memory with them");
     for (const MaybeTensor* t : {&history, &lengths, &repetition, &presence, &frequency, &bias_ids, &bias_values, &allowed})
         if (t->has_value()) at::assert_no_overlap(out, **t);
     rules_into(logits, history, lengths, repetition, repetition_all, presence, presence_all, frequency, frequency_all, bias_ids, bias_values, allowed, out);
