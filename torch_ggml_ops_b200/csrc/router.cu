@@ -609,7 +609,16 @@ static unsigned resident_blocks(int64_t tokens) {
     const unsigned b = token_blocks(tokens);
     return b < 148u * n ? b : 148u * n;
 }
-// balance_kernel's: pairs of every expert, the tokens, the warps' sums
+// balance_kernel's blocks: rounds of those that run at once, so many that no warp adds up more than kBalanceRun tokens in fp32 before the sum joins the whole
+// numbers.  Each token of a run may put a sum off by U / 2, and tokens that are all alike round the same way: in one round 2^28 of 3
+// experts were 3.5e-4 off, so 1.3e-6.
+constexpr int64_t kBalanceRun = 256;
+template <auto KERNEL, size_t SMEM>
+static unsigned balance_blocks(int64_t tokens) {
+    const int64_t at_once = resident_blocks<KERNEL, SMEM>(tokens), run = at_once * kRouterWarps * kBalanceRun;
+    return static_cast<unsigned>((tokens + run - 1) / run * at_once);
+}
+// its shared memory: pairs of every expert, the tokens, the warps' sums
 static constexpr size_t balance_smem(int64_t experts) { return ((kRouterWarps + 1) * experts + 1) * 4; }
 
 // log2(tokens), rounded up
@@ -690,8 +699,8 @@ int tgo_moe_balance_loss(const void* logits, int dtype, int64_t tokens, int64_t 
         constexpr int VPL = decltype(vpl)::value;
         const BalanceArgs a = {logits, tokens, row_stride, static_cast<int>(experts), static_cast<int>(top_k),
                                RowLayout<T, VPL>::whole_chunks(logits, experts, row_stride), expert_ids};
-        if (scoring == TGO_SCORING_SIGMOID) balance_kernel<T, VPL, true><<<resident_blocks<balance_kernel<T, VPL, true>, balance_smem(32 * VPL)>(tokens), kRouterWarps * 32, smem, st>>>(a, sums, loss, counts, coef);
-        else balance_kernel<T, VPL, false><<<resident_blocks<balance_kernel<T, VPL, false>, balance_smem(32 * VPL)>(tokens), kRouterWarps * 32, smem, st>>>(a, sums, loss, counts, coef);
+        if (scoring == TGO_SCORING_SIGMOID) balance_kernel<T, VPL, true><<<balance_blocks<balance_kernel<T, VPL, true>, balance_smem(32 * VPL)>(tokens), kRouterWarps * 32, smem, st>>>(a, sums, loss, counts, coef);
+        else balance_kernel<T, VPL, false><<<balance_blocks<balance_kernel<T, VPL, false>, balance_smem(32 * VPL)>(tokens), kRouterWarps * 32, smem, st>>>(a, sums, loss, counts, coef);
         return launched("balance_kernel launch failed");
     });
 }
