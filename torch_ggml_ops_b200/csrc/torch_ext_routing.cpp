@@ -564,7 +564,7 @@ void rules_into(const Tensor& logits, const MaybeTensor& history, const MaybeTen
     TORCH_CHECK(out.sizes() == logits.sizes() && out.scalar_type() == logits.scalar_type() && out.device() == logits.device(),
                 "out must be a tensor like logits");
     TORCH_CHECK(r.width <= INT32_MAX, "the vocabulary must be below 2^31; got ", r.width);
-    TORCH_CHECK(repetition.has_value() || repetition_all > 0, "repetition_penalty must be positive; got ", repetition_all);
+    TORCH_CHECK(repetition.has_value() || static_cast<float>(repetition_all) > 0, "repetition_penalty must be positive in fp32; got ", repetition_all);
     int64_t history_stride = 0, ids_stride = 0, values_stride = 0, allowed_stride = 0;
     if (history.has_value()) {
         TORCH_CHECK(is_id(*history), "history must have dtype torch.int32 or torch.int64");
