@@ -6,8 +6,8 @@
 //
 // All of it is bound by memory: a token's row is read once and its top_k rows are written (or read) once.  One B200, rows of
 // 2048, top 8, GPU time in a graph (bytes that have to move over it):
-//   dispatch 16384 tokens 116 us (5.2 TB/s; the rows alone 98, 6.2 TB/s), its gradient 93.8 (6.4)
-//   combine 600 tokens 4.4 us, 8192 48.6 (6.2 TB/s), its gradients 97.6 (5.9)
+//   dispatch 16384 tokens 118 us (5.1 TB/s): the sort 13, the rows 105 (5.8 TB/s); its gradient 93.8 (6.4)
+//   combine 600 tokens 4.4 us, 8192 48.6 (6.2 TB/s), its gradients 99 (5.8)
 // A copy runs at 6.4.
 #include "../../include/tgo_mmq.h"
 
@@ -51,6 +51,9 @@ __device__ __forceinline__ uint4 narrow(const float (&f)[8]) {
 // a whole dispatch of 2048-wide rows in one launch / sorted (below), in a graph:
 //   256 experts, top 8     1 token 2.6 / 6.2, 16 2.8 / 7.6, 256 4.8 / 9.6, 512 9.2 / 11.5
 //   1000 experts, top 4    16 2.6 / 10.2, 512 5.2 / 12.3, 1024 9.9 / 14.5;   4096 experts, top 8    512 11.8 / 22.2
+//   256 experts, top 1     256 2.3 / 7.7, 1024 3.5 / 8.9, 2048 6.8 / 10.9, 4096 15.1 / 13.8;   top 32    16 5.8 / 10.3, 128 11.4 / 12.1
+//   1024 experts, top 128  8 18.6 / 22.1, 32 36.1 / 23.9;   top 512    1 55.6 / 57.0, 4 87.9 / 58.6;   top 1024    1 130 / 105, 4 257 / 108
+// The rule looks at the pairs alone, as a caller asks for the workspace by them; past a top_k of 100 or so it is not the faster side.
 constexpr int kFewPairs = 4096;
 constexpr int kMoveWarps = kMoveThreads / 32;
 __global__ void __launch_bounds__(kMoveThreads) dispatch_few_kernel(const uint4* __restrict__ x, const int32_t* __restrict__ ids, int experts, int tokens, int top_k,
@@ -99,7 +102,7 @@ __global__ void __launch_bounds__(kMoveThreads) dispatch_few_kernel(const uint4*
 }
 
 // More pairs: counts per block and expert, their running sums, the rows.  All three use the whole GPU (the sort of
-// routing.cu, for 4096 experts, adds up in one block: 131072 pairs, 256 experts, 25 us; these 13).
+// routing.cu, for 4096 experts, adds up in one block: 131072 pairs, 256 experts, 21.6 us; these 13).
 constexpr int kSortExperts = 1024;
 constexpr int kSortPairs = kMoveThreads;   // pairs of a block
 

@@ -17,7 +17,9 @@
 //
 // Measured on one B200, GPU time in a graph (us), 256 experts, top 8, bf16 (floor: scores in or out at 6.4 TB/s, 5.2 us for 65536 tokens):
 //   router      16 tokens 2.3, 65536 29.4;  gradient 65536 12.3 (normalised)
-//   balance     65536 24;  gradient 65536 22 (floor 10.4)
+//   balance     65536 24;  gradient 65536 22 (floor 10.4);  1000 experts, softmax / sigmoid: bf16 89 / 153, gradient 174 / 298 (floors 20.4, 40.8),
+//               fp32 50 / 118, gradient 92 / 209 (floors 40.8, 81.5), whose 192 to 241 registers leave
+//               one block of 8 warps per SM
 //   fp32: router 8200 tokens 6.8, gradient of the plain probabilities 3.7;  1291 tokens of 1000 experts, top 4, 4.6
 // What bounds the router: instructions (345 per token, 69 % of the issue slots): keys 40, eight choices 50, the scores put in
 // after them 50, softmax and result 60; 40 to 64 warps per SM instead of 32 gain nothing.  Choosing by (score, expert) with two reductions and a search of the registers

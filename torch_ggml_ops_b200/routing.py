@@ -104,7 +104,9 @@ def moe_balance_loss(logits: torch.Tensor, expert_ids: torch.Tensor, *, scoring:
 
     ``expert_ids`` [..., top_k] int32 as ``moe_router`` gives them.  A token all of whose ids are outside the experts
     (padding) takes no part; without any token the loss is 0.  The loss is differentiable with respect to
-    ``logits`` (the counts are constants), once; the same call gives the same bits."""
+    ``logits`` (the counts are constants), once; the same call gives the same bits.  That gradient is of the order of one over
+    the tokens and has the logits' type: of fp16 logits of thousands of tokens it falls among fp16's subnormals, so scale the
+    loss, as one does in fp16, or give the scores in bf16 or fp32."""
     return _ops.moe_balance_loss.default(logits, expert_ids, _scoring(scoring))[:2]
 
 
