@@ -37,6 +37,8 @@ def programs(device):
         "moe_dispatch": (lambda x: tgo.moe_dispatch(x, ids, 8), [half(3, 16)]),
         "moe_combine": (lambda r, v: tgo.moe_combine(r, ids, v), [half(6, 16), f32(3, 2)]),
         "moe_combine_grad": (lambda d, r, v: own.moe_combine_grad(d, r, ids, v, True, True), [half(3, 16), half(6, 16), f32(3, 2)]),
+        "moe_combine_rows_grad": (lambda d, v: own.moe_combine_rows_grad(d, ids, v, 6), [half(3, 16), f32(3, 2)]),
+        "moe_dispatch_grad": (lambda d: own.moe_dispatch_grad(d, ids), [half(6, 16)]),
         "logit_rules": (lambda x, v, a, b, c: tgo.logit_rules(x, bias_ids=ids, bias_values=v, repetition_penalty=a, presence_penalty=b, frequency_penalty=c),
                         [f32(3, 8), f32(3, 2), f32(3), f32(3), f32(3)]),
         "logit_rules_out": (lambda x, v, a, b, c, o: tgo.logit_rules(x, bias_ids=ids, bias_values=v, repetition_penalty=a, presence_penalty=b, frequency_penalty=c,

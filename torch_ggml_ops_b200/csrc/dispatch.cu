@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(kListThreads) count_rows_kernel(const int32_t*
     if (__ldcg(&l.state[1]) == 0) return;
 
     __shared__ int32_t next[256];                 // where a digit's next entry goes
-    __shared__ uint16_t among[kListWarps][256];    // a step's entries of a digit per warp, then in the warps in front
+    __shared__ uint16_t among[kListWarps][256];   // a step's entries of a digit per warp, then in the warps in front
     __shared__ int32_t total;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     long long n = pairs;                          // the first pass looks at all pairs and takes those of rows that are named again
